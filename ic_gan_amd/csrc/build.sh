@@ -5,11 +5,12 @@ HERE="$(cd "$(dirname "${BASH_SOURCE[0]}")" && pwd)"
 OUT="$HERE/../lib"
 mkdir -p "$OUT" "$HERE/obj"
 HIPCC="${HIPCC:-/opt/rocm/bin/hipcc}"
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-value -Wno-sometimes-uninitialized -Wno-uninitialized"
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (the compiler forms them from ordinary float code by itself)
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-unused-value -Wno-sometimes-uninitialized -Wno-uninitialized"
 pids=()
 for src in "$HERE"/*.hip; do
   obj="$HERE/obj/$(basename "${src%.hip}").o"
-  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$HERE/icg_common.h" -nt "$obj" ] || [ "$HERE/../../include/icgan_hip.h" -nt "$obj" ]; then
+  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ -n "$(find "$HERE" \( -name '*.h' -o -name build.sh \) -newer "$obj")" ] || [ "$HERE/../../include/icgan_hip.h" -nt "$obj" ]; then
     ( $HIPCC $FLAGS -c "$src" -o "$obj" ) &
     pids+=($!)
   fi

@@ -12,7 +12,7 @@
 //
 // Warp specialisation (12 waves = 768 threads, 3 per SIMD):
 //   * waves 8..11, PRODUCERS: lane = (tile, channel PAIR) of a 32-channel chunk; the 6 x 6 (4 x 4 source pixels, upsample-fused
-//     form) window lives in registers as float2: BN / ccbn affine + ReLU + zero padding, B^T d B with v_pk_* arithmetic, the 36
+//     form) window lives in registers as float2: BN / ccbn affine + ReLU + zero padding, B^T d B on channel pairs, the 36
 //     values go to LDS in the MFMA operand order (ds_write_b64, conflict-free through an XOR of the tile index with the channel
 //     quad); optionally also to HBM as the V planes the weight gradient wants (icg_conv2d_wino4_wgrad_from_v).  The window is
 //     REFILLED IN PLACE: the second 1-D pass retires it line by line and each retired line's registers are loaded at once with
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256) void icg_fwino_pack_kernel(const float* __rest
   }
 }
 
-// transforms on channel PAIRS (v_pk_* arithmetic): the producers' instruction count is what they cost the MFMA waves they share a
+// transforms on channel PAIRS: the producers' instruction count is what they cost the MFMA waves they share a
 // SIMD with
 // FWINO_SCALAR (measurement builds, tools/build_dbg.sh FWS): the same arithmetic on two plain floats (compile with
 // -fno-slp-vectorize) -- packed fp32 VALU beside MFMAs has an issue cost of its own (MI355X_MICROARCH.md)

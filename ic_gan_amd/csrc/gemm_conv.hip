@@ -661,16 +661,14 @@ __device__ __forceinline__ void icg_gemm_body(const GemmP& p) {
         if (FLUSH && t == 0) {
           // fold the finished chain into the second level, restart from C = 0 (inline constant: no register zeroing)
           asm volatile("" : "+a"(acc[j]));    // ... and the accumulator -> VGPR copies must not be hoisted to the loop head
-          // 8 packed adds (v_pk_add_f32) per column tile, written as asm: the vector add is otherwise legalised into 13 scalar
-          // + 1.5 packed adds per tile, and -- being pure, with a result nobody reads before the next flush -- sunk to the
-          // end of the loop body, which keeps all 16*TN accumulator copies live in VGPRs meanwhile
+          // 16 adds per column tile, written as asm: the C++ adds -- being pure, with a result nobody reads before the next flush --
+          // are sunk to the end of the loop body, which keeps all 16*TN accumulator copies live in VGPRs meanwhile
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
-            f32x2 a2 = {acc[j][2 * r], acc[j][2 * r + 1]};
-            f32x2 b2 = {acc2[j][2 * r], acc2[j][2 * r + 1]};
-            asm volatile("v_pk_add_f32 %0, %0, %1" : "+v"(b2) : "v"(a2));
-            acc2[j][2 * r] = b2.x;
-            acc2[j][2 * r + 1] = b2.y;
+            float b0 = acc2[j][2 * r], b1 = acc2[j][2 * r + 1];
+            asm volatile("v_add_f32 %0, %0, %2\n\tv_add_f32 %1, %1, %3" : "+&v"(b0), "+&v"(b1) : "v"(acc[j][2 * r]), "v"(acc[j][2 * r + 1]));
+            acc2[j][2 * r] = b0;
+            acc2[j][2 * r + 1] = b1;
           }
           f32x16 zero;
 #pragma unroll
@@ -925,11 +923,10 @@ __device__ __forceinline__ void icg_planes_body(const GemmP& p) {
           } else {
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-              f32x2 a2 = {acc[j][2 * r], acc[j][2 * r + 1]};
-              f32x2 b2 = {acc2[j][2 * r], acc2[j][2 * r + 1]};
-              asm volatile("v_pk_add_f32 %0, %0, %1" : "+v"(b2) : "v"(a2));
-              acc2[j][2 * r] = b2.x;
-              acc2[j][2 * r + 1] = b2.y;
+              float b0 = acc2[j][2 * r], b1 = acc2[j][2 * r + 1];
+              asm volatile("v_add_f32 %0, %0, %2\n\tv_add_f32 %1, %1, %3" : "+&v"(b0), "+&v"(b1) : "v"(acc[j][2 * r]), "v"(acc[j][2 * r + 1]));
+              acc2[j][2 * r] = b0;
+              acc2[j][2 * r + 1] = b1;
             }
           }
           f32x16 zero;
@@ -999,7 +996,9 @@ __device__ __forceinline__ void icg_planes_body(const GemmP& p) {
         f32x2 c2 = {acc[j][2 * r], acc[j][2 * r + 1]};
         if (BLK) {
           f32x2 b2 = {acc2[j][2 * r], acc2[j][2 * r + 1]};
-          asm volatile("v_pk_add_f32 %0, %0, %1" : "+v"(c2) : "v"(b2));
+          float c0 = c2.x, c1 = c2.y;
+          asm volatile("v_add_f32 %0, %0, %2\n\tv_add_f32 %1, %1, %3" : "+&v"(c0), "+&v"(c1) : "v"(b2.x), "v"(b2.y));
+          c2 = f32x2{c0, c1};
         } else {
           asm volatile("" : "+v"(c2));
         }

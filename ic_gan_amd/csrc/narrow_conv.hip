@@ -14,7 +14,7 @@
 #define NC_ROWS 32      // rows of a column segment (2 halo rows per segment are re-read)
 
 typedef float th_f32x16 __attribute__((ext_vector_type(16)));   // MFMA accumulator tile
-typedef float nc_v2 __attribute__((ext_vector_type(2)));      // v_pk_fma_f32: two fp32 FMAs per lane and issue slot
+typedef float nc_v2 __attribute__((ext_vector_type(2)));      // a pair of channels
 __device__ __forceinline__ nc_v2 nc_lo(const float4& v) { return nc_v2{v.x, v.y}; }
 __device__ __forceinline__ nc_v2 nc_hi(const float4& v) { return nc_v2{v.z, v.w}; }
 
