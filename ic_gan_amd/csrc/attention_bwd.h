@@ -1,0 +1,313 @@
+// Gradient kernels of csrc/attention.h (internal header, included once per element type).  The probabilities are computed again from the
+// scores and the forward's l_i.  Two kernels, each owning what it sums -- keys (dk, dv) or queries (dq) -- so no atomics and the same bits on
+// every run; the price is that scores and do . v are formed twice (7 products instead of 5).
+#pragma once
+#include "attention.h"
+
+// D_i = do_i . o_i, |do_i| and the exponent's offset, a row per 32 lanes; rows in memory order
+template <typename T>
+__global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, float* stat) {
+  const int64_t rows = (int64_t)p.B * p.H * p.Lq, i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int l = threadIdx.x & 31;
+  if (i >= rows) return;
+  const int64_t bq = i / p.H;
+  const int hq = (int)(i - bq * p.H);
+  const int64_t b = bq / p.Lq, qi = bq - b * p.Lq;
+  const T* o = reinterpret_cast<const T*>(p.o) + i * p.dv;
+  const T* g = reinterpret_cast<const T*>(p.dout) + b * p.do_sb + qi * p.do_sl + hq * p.do_sh;
+  constexpr int PER = 16 / (int)sizeof(T);
+  float dot = 0.f, sq = 0.f;
+  for (int c = l; c * PER < p.dv; c += 32) {
+    const at_u4 a = at_load_chunk<T>(o, c, p.dv, (p.dv * sizeof(T)) % 16 == 0), e = at_load_chunk<T>(g, c, p.dv, p.do_vec);
+    T x[PER], y[PER];
+    __builtin_memcpy(x, &a, 16);
+    __builtin_memcpy(y, &e, 16);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) dot = __builtin_fmaf((float)x[j], (float)y[j], dot), sq = __builtin_fmaf((float)y[j], (float)y[j], sq);
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor(dot, s, 64), sq += __shfl_xor(sq, s, 64);
+  if (l == 0) {
+    const int64_t row = (b * p.H + hq) * p.Lq + qi;
+    const float lse = p.lse[row];
+    stat[row] = lse == -INFINITY ? INFINITY : __builtin_fmaf(lse, AT_LOG2E, -(float)at_type<T>::P_SHIFT);   // (a row that saw no key: p = exp2(s - inf) = 0)
+    stat[rows + row] = dot;
+    stat[2 * rows + row] = sqrtf(sq);
+  }
+}
+
+// the power of two that brings a norm to [1, 2); 1 where there is none
+__device__ __forceinline__ float at_to_one(float norm) {
+  const unsigned e = (__float_as_uint(norm) >> 23) & 255u;
+  return e == 0u || e >= 254u ? 1.f : __uint_as_float((254u - e) << 23);
+}
+template <typename T>
+__device__ __forceinline__ float at_ds(float pr, float dp, float s, float delta_s) {
+  const float x = pr * __builtin_fmaf(dp, s, -delta_s);
+  if constexpr (at_type<T>::SCALED) return __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f);
+  return x;
+}
+
+// dq: a workgroup owns 128 queries of one head (a wave 32, as columns) and streams the keys
+template <typename T, int DP, int DVP>
+__global__ __launch_bounds__(256) void icg_attention_dq_kernel(AttnP p) {
+  typedef at_type<T> X;
+  typedef typename X::frag frag;
+  constexpr int KT = sizeof(T) == 4 ? 32 : 64, KBYTES = KT * at_tile<T, DP>::STRIDE, SLOT = KBYTES + KT * at_tile<T, DVP>::STRIDE;
+  __shared__ __attribute__((aligned(64))) char lds[2 * SLOT];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 31, h = lane >> 5;
+  const int64_t item = at_work_item(p.work);
+  int tile = (int)(item % p.tiles);
+  const int64_t bh = item / p.tiles;
+  const int b = (int)(bh / p.H), hq = (int)(bh - (int64_t)b * p.H), hk = hq / p.G;
+  if (p.causal) tile = p.tiles - 1 - tile;
+  const int qi = 128 * tile + 32 * wv + m;
+  const bool valid = qi < p.Lq;
+  const int keys = at_keys(p, b), start = at_start(p, b);
+  const int last = !valid ? -1 : (p.causal ? min(keys - 1, start + qi) : keys - 1);
+  const int kend = p.causal ? min(keys, start + min(p.Lq - 1, 128 * tile + 127) + 1) : keys;
+
+  frag qf[DP / X::KSTEP], gf[DVP / X::KSTEP];
+  at_own<T, DP>(qf, reinterpret_cast<const T*>(p.q) + b * p.q_sb + qi * p.q_sl + hq * p.q_sh, valid, p.d, p.q_vec, h);
+  at_own<T, DVP>(gf, reinterpret_cast<const T*>(p.dout) + b * p.do_sb + qi * p.do_sl + hq * p.do_sh, valid, p.dv, p.do_vec, h);
+  const int64_t rows = (int64_t)p.B * p.H * p.Lq, row = ((int64_t)b * p.H + hq) * p.Lq + qi;
+  const float lse2 = valid ? p.stat[row] : INFINITY;
+  const float s1 = X::SCALED && valid ? at_to_one(p.stat[2 * rows + row]) : 1.f;
+  const float delta = valid ? p.stat[rows + row] * s1 : 0.f;
+  const T* kb = reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* vb = reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  const at_reader<T, DP> kr(lane);
+  const at_reader<T, DVP> vr(lane);
+  const float scl = p.scale * AT_LOG2E;
+
+  at_f16v acc[DP / 32];
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[c][i] = 0.f;
+  at_stage<T, DP, KT, 256> ks;
+  at_stage<T, DVP, KT, 256> vs;
+  auto fetch = [&](int j) {
+    ks.fetch(kb, p.k_sl, j, kend, p.d, p.k_vec, tid);
+    vs.fetch(vb, p.v_sl, j, kend, p.dv, p.v_vec, tid);
+  };
+  auto put = [&](int cur) {
+    ks.put(lds + cur * SLOT, tid);
+    vs.put(lds + cur * SLOT + KBYTES, tid);
+  };
+  int cur = 0;
+  if (kend > 0) {
+    fetch(0);
+    put(0);
+    if (KT < kend) fetch(KT);
+    __syncthreads();
+  }
+  for (int j0 = 0; j0 < kend; j0 += KT) {
+    const char* kt = lds + cur * SLOT;
+    const char* vt = kt + KBYTES;
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u) {
+      at_f16v s, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = 0.f, dp[i] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DP / X::KSTEP; ++t) s = X::mma(kr.row_frag(kt, 32 * u, t), qf[t], s);
+#pragma unroll
+      for (int t = 0; t < DVP / X::KSTEP; ++t) dp = X::mma(vr.row_frag(vt, 32 * u, t), gf[t], dp);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = at_ds<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scl, -lse2)), dp[i], s1, delta);
+      if (__any(j0 + 32 * u + 31 > last)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = j0 + 32 * u + at_row_of(i, h) > last ? 0.f : s[i];
+      }
+      // ds is rounded to the inputs' type for the matrix product: half a step each, summed over the keys in 32 bits
+#pragma unroll
+      for (int q = 0; q < 32 / X::KSTEP; ++q) {
+        const frag sf = X::pack(s, q);
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) acc[c] = X::mma(kr.col_frag(kt, 32 * u, c, q), sf, acc[c]);
+      }
+    }
+    if (j0 + KT < kend) {
+      cur ^= 1;
+      put(cur);
+      if (j0 + 2 * KT < kend) fetch(j0 + 2 * KT);
+      __syncthreads();
+    }
+  }
+  if (!valid) return;
+  const float f = p.scale * (1.f / (1 << X::P_SHIFT)) / s1;
+  T* out = reinterpret_cast<T*>(p.dq) + (((int64_t)b * p.Lq + qi) * p.H + hq) * p.d;
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      at_store4<T>(out, 32 * c + 8 * g + 4 * h, p.d, acc[c][4 * g] * f, acc[c][4 * g + 1] * f, acc[c][4 * g + 2] * f, acc[c][4 * g + 3] * f);
+}
+
+// dk, dv: a workgroup owns 128 keys of one key head (a wave 32, as columns) and streams the queries of every head of the group, so the
+// gradient of a shared head is summed in registers
+template <typename T, int DP, int DVP>
+__global__ __launch_bounds__(256) void icg_attention_dkv_kernel(AttnP p) {
+  typedef at_type<T> X;
+  typedef typename X::frag frag;
+  constexpr int QT = 32, QBYTES = QT * at_tile<T, DP>::STRIDE, GBYTES = QT * at_tile<T, DVP>::STRIDE, SLOT = QBYTES + GBYTES + 2 * QT * 4;
+  __shared__ __attribute__((aligned(64))) char lds[2 * SLOT];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 31, h = lane >> 5;
+  const int64_t item = at_work_item(p.work);
+  const int tile = (int)(item % p.tiles);
+  const int64_t bh = item / p.tiles;
+  const int Hk = p.H / p.G, b = (int)(bh / Hk), hk = (int)(bh - (int64_t)b * Hk);
+  const int j = 128 * tile + 32 * wv + m;
+  const int keys = at_keys(p, b), start = at_start(p, b);
+  const bool valid = j < keys;
+  const int64_t rows = (int64_t)p.B * p.H * p.Lq, row_b = ((int64_t)b * p.H + hk * p.G) * p.Lq;
+
+  frag kf[DP / X::KSTEP], vf[DVP / X::KSTEP];
+  at_own<T, DP>(kf, reinterpret_cast<const T*>(p.k) + b * p.k_sb + j * p.k_sl + hk * p.k_sh, valid, p.d, p.k_vec, h);
+  at_own<T, DVP>(vf, reinterpret_cast<const T*>(p.v) + b * p.v_sb + j * p.v_sl + hk * p.v_sh, valid, p.dv, p.v_vec, h);
+  const at_reader<T, DP> qr(lane);
+  const at_reader<T, DVP> gr(lane);
+  const float scl = p.scale * AT_LOG2E;
+
+  float s1 = 1.f;
+  if constexpr (X::SCALED) {                             // one scale for everything that is summed here
+    float* red = reinterpret_cast<float*>(lds);
+    float n = 0.f;
+    for (int64_t i = tid; i < (int64_t)p.G * p.Lq; i += 256) n = fmaxf(n, p.stat[2 * rows + row_b + i]);
+    n = wave_max(n);
+    if (lane == 0) red[wv] = n;
+    __syncthreads();
+    s1 = at_to_one(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    __syncthreads();
+  }
+
+  at_f16v dk[DP / 32], dv[DVP / 32];
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dk[c][i] = 0.f;
+#pragma unroll
+  for (int c = 0; c < DVP / 32; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dv[c][i] = 0.f;
+
+  // query i sees key j from i = j - start on
+  const int i0 = p.causal ? max(0, 128 * tile - start) / QT : 0;
+  const int per = max(0, (p.Lq + QT - 1) / QT - i0), n = 128 * tile < keys ? p.G * per : 0;
+  at_stage<T, DP, QT, 256> qs;
+  at_stage<T, DVP, QT, 256> gs;
+  float st = 0.f;                                        // threads 0 .. QT - 1: l_i, QT .. 2 QT - 1: D_i
+  int fg = 0, ft = 0;                                    // head and tile of the next fetch
+  auto fetch = [&]() {
+    const int r0 = (i0 + ft) * QT, hq = hk * p.G + fg;
+    qs.fetch(reinterpret_cast<const T*>(p.q) + b * p.q_sb + hq * p.q_sh, p.q_sl, r0, p.Lq, p.d, p.q_vec, tid);
+    gs.fetch(reinterpret_cast<const T*>(p.dout) + b * p.do_sb + hq * p.do_sh, p.do_sl, r0, p.Lq, p.dv, p.do_vec, tid);
+    if (tid < 2 * QT) {
+      const int i = r0 + (tid & (QT - 1));
+      const int64_t at = row_b + (int64_t)fg * p.Lq + i;
+      st = tid < QT ? (i < p.Lq ? p.stat[at] : INFINITY) : (i < p.Lq ? p.stat[rows + at] * s1 : 0.f);
+    }
+    if (++ft == per) ft = 0, ++fg;
+  };
+  auto put = [&](int cur) {
+    char* at = lds + cur * SLOT;
+    qs.put(at, tid);
+    gs.put(at + QBYTES, tid);
+    if (tid < 2 * QT) reinterpret_cast<float*>(at + QBYTES + GBYTES)[tid] = st;
+  };
+  int cur = 0, t0 = 0;                                   // tile of the current one within its head
+  if (n > 0) {
+    fetch();
+    put(0);
+    if (n > 1) fetch();
+    __syncthreads();
+  }
+  for (int it = 0; it < n; ++it) {
+    const char* qt = lds + cur * SLOT;
+    const char* gt = qt + QBYTES;
+    const float* stat = reinterpret_cast<const float*>(gt + GBYTES);
+    at_f16v s, dp;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f, dp[i] = 0.f;
+#pragma unroll
+    for (int t = 0; t < DP / X::KSTEP; ++t) s = X::mma(qr.row_frag(qt, 0, t), kf[t], s);
+#pragma unroll
+    for (int t = 0; t < DVP / X::KSTEP; ++t) dp = X::mma(gr.row_frag(gt, 0, t), vf[t], dp);
+    const int first = valid ? (p.causal ? j - start : -(1 << 30)) : 0x7fffffff;       // the first query that sees this lane's key
+    const int r0 = (i0 + t0) * QT;
+    const bool edge = __any(r0 < first);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const at_f4 l4 = *reinterpret_cast<const at_f4*>(stat + 8 * g + 4 * h), d4 = *reinterpret_cast<const at_f4*>(stat + QT + 8 * g + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * g + e;
+        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scl, -l4[e]));
+        dp[i] = at_ds<T>(s[i], dp[i], s1, d4[e]);
+      }
+    }
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool off = r0 + at_row_of(i, h) < first;
+        s[i] = off ? 0.f : s[i];
+        dp[i] = off ? 0.f : dp[i];
+      }
+    }
+    // p and ds are rounded to the inputs' type for the matrix products: half a step each, summed over the queries in 32 bits
+#pragma unroll
+    for (int q = 0; q < 32 / X::KSTEP; ++q) {
+      const frag pf = X::pack(s, q), sf = X::pack(dp, q);
+#pragma unroll
+      for (int c = 0; c < DVP / 32; ++c) dv[c] = X::mma(gr.col_frag(gt, 0, c, q), pf, dv[c]);
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) dk[c] = X::mma(qr.col_frag(qt, 0, c, q), sf, dk[c]);
+    }
+    if (++t0 == per) t0 = 0;
+    if (it + 1 < n) {
+      cur ^= 1;
+      put(cur);
+      if (it + 2 < n) fetch();
+      __syncthreads();
+    }
+  }
+  if (j >= p.Lk) return;                                 // (keys from k_lens on have no gradient: their sums are zero)
+  const float fv = 1.f / (1 << X::P_SHIFT), fk = p.scale * fv / s1;
+  T* dk_out = reinterpret_cast<T*>(p.dk) + (((int64_t)b * p.Lk + j) * Hk + hk) * p.d;
+  T* dv_out = reinterpret_cast<T*>(p.dv_out) + (((int64_t)b * p.Lk + j) * Hk + hk) * p.dv;
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      at_store4<T>(dk_out, 32 * c + 8 * g + 4 * h, p.d, dk[c][4 * g] * fk, dk[c][4 * g + 1] * fk, dk[c][4 * g + 2] * fk, dk[c][4 * g + 3] * fk);
+#pragma unroll
+  for (int c = 0; c < DVP / 32; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      at_store4<T>(dv_out, 32 * c + 8 * g + 4 * h, p.dv, dv[c][4 * g] * fv, dv[c][4 * g + 1] * fv, dv[c][4 * g + 2] * fv, dv[c][4 * g + 3] * fv);
+}
+
+template <typename T>
+int at_bwd(const AttnP& in, float* stat, hipStream_t st) {
+  AttnP p = in;
+  p.stat = stat;
+  hipLaunchKernelGGL((icg_attention_rowstat_kernel<T>), dim3((unsigned)icg_cdiv((int64_t)p.B * p.H * p.Lq, 8)), dim3(256), 0, st, p, stat);
+  if (const int e = icg_check_launch()) return e;
+  AttnP pk = p;
+  pk.tiles = (int)icg_cdiv(p.Lk, 128);
+  pk.work = (int64_t)p.B * (p.H / p.G) * pk.tiles;
+  p.tiles = (int)icg_cdiv(p.Lq, 128);
+  p.work = (int64_t)p.B * p.H * p.tiles;
+#define AT_RUN(DP, DVP)                                                                                                 \
+  do {                                                                                                                  \
+    hipLaunchKernelGGL((icg_attention_dkv_kernel<T, DP, DVP>), dim3((unsigned)pk.work), dim3(256), 0, st, pk);          \
+    if (const int e = icg_check_launch()) return e;                                                                     \
+    hipLaunchKernelGGL((icg_attention_dq_kernel<T, DP, DVP>), dim3((unsigned)p.work), dim3(256), 0, st, p);             \
+  } while (0)
+  AT_FOR_HEAD(p.d, p.dv, AT_RUN)
+#undef AT_RUN
+  return icg_check_launch();
+}

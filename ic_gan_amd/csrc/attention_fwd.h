@@ -1,0 +1,277 @@
+// Forward kernels of csrc/attention.h: one pass over the keys with the running maximum and sum of the softmax (internal header, included
+// once per element type).
+#pragma once
+#include "attention.h"
+
+template <typename T, bool TOKENS>
+struct at_fwd_shape {
+  // ROWS: 4 waves, 32 queries of one head each, all of them against every streamed tile of KT keys.
+  // TOKENS (few queries): ONE tile of 32 rows, the (query, head) pairs that share a key head; each wave takes 32 of the KT keys, so a
+  // tile is read once for the whole group and the waves' results are joined at the end.
+  static constexpr int WAVES = TOKENS && sizeof(T) == 4 ? 2 : 4;
+  static constexpr int THREADS = 64 * WAVES;
+  static constexpr int KT = TOKENS ? 32 * WAVES : (sizeof(T) == 4 ? 32 : 64);
+  static constexpr int SUB = TOKENS ? 1 : KT / 32;      // 32-key tiles of one wave
+  static constexpr int BUFFERS = TOKENS ? 1 : 2;
+};
+
+template <typename T, int DP, int DVP, bool TOKENS>
+__global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS)) void icg_attention_fwd_kernel(AttnP p) {
+  typedef at_fwd_shape<T, TOKENS> S;
+  typedef at_type<T> X;
+  typedef typename X::frag frag;
+  typedef at_tile<T, DP> KTile;
+  typedef at_tile<T, DVP> VTile;
+  constexpr int KBYTES = S::KT * KTile::STRIDE, VBYTES = S::KT * VTile::STRIDE, SLOT = KBYTES + VBYTES;
+  constexpr int JOIN = TOKENS ? 32 * DVP * 4 + 2 * S::WAVES * 32 * 4 : 0;
+  constexpr int LDS = S::BUFFERS * SLOT > JOIN ? S::BUFFERS * SLOT : JOIN;
+  constexpr int NV = DVP / 32;
+  __shared__ __attribute__((aligned(64))) char lds[LDS];
+
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 31, h = lane >> 5;
+  int64_t item = at_work_item(p.work);
+  const int split = (int)(item % p.nsplit);
+  item /= p.nsplit;
+  int tile = (int)(item % p.tiles);
+  const int64_t bh = item / p.tiles;                     // (batch, query head), or (batch, key head) for TOKENS
+  const int heads = TOKENS ? p.H / p.G : p.H;
+  const int b = (int)(bh / heads), head = (int)(bh - (int64_t)b * heads);
+  if (!TOKENS && p.causal) tile = p.tiles - 1 - tile;    // the long rows of a causal triangle first
+
+  int qi, hq, qi_last;
+  bool valid;
+  if constexpr (TOKENS) {
+    const int r = 32 * tile + m;
+    valid = r < p.Lq * p.G;
+    qi = r / p.G;
+    hq = head * p.G + (r - qi * p.G);
+    qi_last = min(p.Lq - 1, (32 * tile + 31) / p.G);
+  } else {
+    qi = 128 * tile + 32 * wv + m;
+    valid = qi < p.Lq;
+    hq = head;
+    qi_last = min(p.Lq - 1, 128 * tile + 127);
+  }
+  const int hk = TOKENS ? head : head / p.G;
+  const int keys = at_keys(p, b), start = at_start(p, b);
+  const int last = !valid ? -1 : (p.causal ? min(keys - 1, start + qi) : keys - 1);      // the last key that this lane's query sees
+  int kend = p.causal ? min(keys, start + qi_last + 1) : keys;
+  int k0 = 0;
+  if (p.nsplit > 1) {
+    k0 = split * p.keys_per_split;
+    kend = min(kend, k0 + p.keys_per_split);
+  }
+
+  frag qf[DP / X::KSTEP];
+  at_own<T, DP>(qf, reinterpret_cast<const T*>(p.q) + b * p.q_sb + qi * p.q_sl + hq * p.q_sh, valid, p.d, p.q_vec, h);
+  const T* kb = reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* vb = reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  const at_reader<T, DP> kr(lane);
+  const at_reader<T, DVP> vr(lane);
+
+  at_f16v o[NV];
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
+  float mx = AT_LOWEST, sum = 0.f;                       // running maximum (of s log2 e) and this half's part of the sum
+  const float scl = p.scale * AT_LOG2E;
+
+  at_stage<T, DP, S::KT, S::THREADS> ks;
+  at_stage<T, DVP, S::KT, S::THREADS> vs;
+  if (k0 < kend) {
+    ks.fetch(kb, p.k_sl, k0, kend, p.d, p.k_vec, tid);
+    vs.fetch(vb, p.v_sl, k0, kend, p.dv, p.v_vec, tid);
+  }
+  int cur = 0;
+  if (S::BUFFERS == 2 && k0 < kend) {
+    ks.put(lds, tid);
+    vs.put(lds + KBYTES, tid);
+    if (k0 + S::KT < kend) {
+      ks.fetch(kb, p.k_sl, k0 + S::KT, kend, p.d, p.k_vec, tid);
+      vs.fetch(vb, p.v_sl, k0 + S::KT, kend, p.dv, p.v_vec, tid);
+    }
+    __syncthreads();
+  }
+  for (int j0 = k0; j0 < kend; j0 += S::KT) {
+    if constexpr (S::BUFFERS == 1) {
+      __syncthreads();                                   // every wave has read the tile before
+      ks.put(lds, tid);
+      vs.put(lds + KBYTES, tid);
+      if (j0 + S::KT < kend) {
+        ks.fetch(kb, p.k_sl, j0 + S::KT, kend, p.d, p.k_vec, tid);
+        vs.fetch(vb, p.v_sl, j0 + S::KT, kend, p.dv, p.v_vec, tid);
+      }
+      __syncthreads();
+    }
+    const char* kt = lds + cur * SLOT;
+    const char* vt = kt + KBYTES;
+    const int sub0 = TOKENS ? 32 * wv : 0;
+    at_f16v s[S::SUB];
+#pragma unroll
+    for (int u = 0; u < S::SUB; ++u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DP / X::KSTEP; ++t) s[u] = X::mma(kr.row_frag(kt, sub0 + 32 * u, t), qf[t], s[u]);
+    }
+    const int jw = j0 + sub0;
+    if (__any(jw + 32 * S::SUB - 1 > last)) {
+#pragma unroll
+      for (int u = 0; u < S::SUB; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] = jw + 32 * u + at_row_of(i, h) > last ? -INFINITY : s[u][i];
+    }
+    float t = s[0][0];
+#pragma unroll
+    for (int u = 0; u < S::SUB; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t = fmaxf(t, s[u][i]);
+    t = at_other_half_max(t) * scl;
+    // the sums are brought to a new maximum only when it grew by more than 2^8: p stays below 256, exact in the products' types
+    if (__any(t > mx + 8.f)) {
+      const float next = fmaxf(mx, t), a = __builtin_amdgcn_exp2f(mx - next);
+      mx = next;
+      sum *= a;
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[c][i] *= a;
+    }
+#pragma unroll
+    for (int u = 0; u < S::SUB; ++u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], scl, -mx));
+      float a = 0.f, c = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) a += s[u][i], c += s[u][i + 1];
+      sum += a + c;
+      // p is rounded to the inputs' type for the matrix product (half a step of values whose errors average out over the keys); its sum is not
+#pragma unroll
+      for (int q = 0; q < 32 / X::KSTEP; ++q) {
+        const frag pf = X::pack(s[u], q);
+#pragma unroll
+        for (int cc = 0; cc < NV; ++cc) o[cc] = X::mma(vr.col_frag(vt, sub0 + 32 * u, cc, q), pf, o[cc]);
+      }
+    }
+    if constexpr (S::BUFFERS == 2) {
+      if (j0 + S::KT < kend) {
+        cur ^= 1;
+        ks.put(lds + cur * SLOT, tid);
+        vs.put(lds + cur * SLOT + KBYTES, tid);
+        if (j0 + 2 * S::KT < kend) {
+          ks.fetch(kb, p.k_sl, j0 + 2 * S::KT, kend, p.d, p.k_vec, tid);
+          vs.fetch(vb, p.v_sl, j0 + 2 * S::KT, kend, p.dv, p.v_vec, tid);
+        }
+        __syncthreads();
+      }
+    }
+  }
+  sum = at_both_halves_sum(sum);
+
+  if constexpr (TOKENS) {                                // join the waves in a fixed order
+    float* joined = reinterpret_cast<float*>(lds);       // [32 rows][DVP], then the waves' maxima and sums
+    float* stat = joined + 32 * DVP;
+    __syncthreads();
+    if (h == 0) {
+      stat[(2 * wv) * 32 + m] = mx;
+      stat[(2 * wv + 1) * 32 + m] = sum;
+    }
+    __syncthreads();
+    float all = stat[m];
+#pragma unroll
+    for (int w = 1; w < S::WAVES; ++w) all = fmaxf(all, stat[2 * w * 32 + m]);
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < S::WAVES; ++w) sum += stat[(2 * w + 1) * 32 + m] * __builtin_amdgcn_exp2f(stat[2 * w * 32 + m] - all);
+    const float a = __builtin_amdgcn_exp2f(mx - all);
+    mx = all;
+#pragma unroll
+    for (int w = 0; w < S::WAVES; ++w) {
+      if (wv == w) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float* at = joined + (32 * c + at_row_of(i, h)) * 32 + m;      // (column-major: the lanes of a half on different banks)
+            *at = w == 0 ? o[c][i] * a : *at + o[c][i] * a;
+          }
+      }
+      __syncthreads();
+    }
+    // wave w takes the columns of tiles c = w, w + WAVES, ...
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+      if (c % S::WAVES == wv)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[c][i] = joined[(32 * c + at_row_of(i, h)) * 32 + m];
+  }
+  if (!valid) return;
+  const int64_t row = ((int64_t)b * p.H + hq) * p.Lq + qi;
+  const bool writes_stat = h == 0 && (!TOKENS || wv == 0);
+  if (p.nsplit > 1) {
+    const int64_t rows = (int64_t)p.B * p.H * p.Lq;
+    if (writes_stat) reinterpret_cast<at_f2*>(p.part + p.nsplit * rows * p.dv)[split * rows + row] = at_f2{mx, sum};
+    if (sum == 0.f) return;                              // (the join does not read the sums of a split that saw no key)
+    float* out = p.part + (split * rows + row) * p.dv;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+      if (!TOKENS || c % S::WAVES == wv)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          at_store4<float>(out, 32 * c + 8 * g + 4 * h, p.dv, o[c][4 * g], o[c][4 * g + 1], o[c][4 * g + 2], o[c][4 * g + 3]);
+    return;
+  }
+  if (writes_stat) p.lse[row] = sum == 0.f ? -INFINITY : mx * AT_LN2 + __logf(sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;        // a row that sees no key is zero
+  T* out = reinterpret_cast<T*>(p.o) + (((int64_t)b * p.Lq + qi) * p.H + hq) * p.dv;
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+    if (!TOKENS || c % S::WAVES == wv)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        at_store4<T>(out, 32 * c + 8 * g + 4 * h, p.dv, o[c][4 * g] * inv, o[c][4 * g + 1] * inv, o[c][4 * g + 2] * inv, o[c][4 * g + 3] * inv);
+}
+
+// joins the splits of one row: 64 lanes, 4 columns each, splits in order
+template <typename T>
+__global__ __launch_bounds__(64) void icg_attention_join_kernel(AttnP p) {
+  const int64_t rows = (int64_t)p.B * p.H * p.Lq, row = blockIdx.x;
+  const at_f2* stat = reinterpret_cast<const at_f2*>(p.part + p.nsplit * rows * p.dv) + row;
+  float mx = AT_LOWEST;
+  for (int s = 0; s < p.nsplit; ++s) mx = fmaxf(mx, stat[s * rows][0]);
+  float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  const int c = 4 * threadIdx.x;
+  for (int s = 0; s < p.nsplit; ++s) {
+    const at_f2 ms = stat[s * rows];
+    if (ms[1] == 0.f) continue;
+    const float a = __builtin_amdgcn_exp2f(ms[0] - mx);
+    sum += ms[1] * a;
+    const float* in = p.part + (s * rows + row) * p.dv + c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) if (c + j < p.dv) o[j] += in[j] * a;
+  }
+  if (threadIdx.x == 0) p.lse[row] = sum == 0.f ? -INFINITY : mx * AT_LN2 + __logf(sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t bh = row / p.Lq, qi = row - bh * p.Lq, b = bh / p.H, hq = bh - b * p.H;
+  T* out = reinterpret_cast<T*>(p.o) + ((b * p.Lq + qi) * p.H + hq) * p.dv;
+  if (c < p.dv) at_store4<T>(out, c, p.dv, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+}
+
+template <typename T>
+int at_fwd(const AttnP& p, bool tokens, hipStream_t st) {
+#define AT_RUN(DP, DVP)                                                                                                                    \
+  do {                                                                                                                                     \
+    if (tokens) hipLaunchKernelGGL((icg_attention_fwd_kernel<T, DP, DVP, true>), dim3((unsigned)p.work), dim3(at_fwd_shape<T, true>::THREADS), 0, st, p); \
+    else hipLaunchKernelGGL((icg_attention_fwd_kernel<T, DP, DVP, false>), dim3((unsigned)p.work), dim3(at_fwd_shape<T, false>::THREADS), 0, st, p);      \
+  } while (0)
+  AT_FOR_HEAD(p.d, p.dv, AT_RUN)
+#undef AT_RUN
+  if (const int e = icg_check_launch()) return e;
+  if (p.nsplit > 1) {
+    hipLaunchKernelGGL((icg_attention_join_kernel<T>), dim3((unsigned)((int64_t)p.B * p.H * p.Lq)), dim3(64), 0, st, p);
+    return icg_check_launch();
+  }
+  return ICG_OK;
+}

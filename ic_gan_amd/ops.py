@@ -8,6 +8,7 @@ is what the kernels address; `_cl` makes that true at module boundaries.
 """
 from __future__ import annotations
 
+import contextlib
 import os
 from dataclasses import dataclass, replace
 from typing import Optional
@@ -15,6 +16,7 @@ from typing import Optional
 import torch
 import torch.distributed as dist
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -1313,6 +1315,118 @@ class AttnOutFn(Function):
                 dweight = _sn_backward(dw_hwio, None, sn, ctx.like)
             dgamma = dgamma.view(ctx.gshape) if need[3] else None
         return da, (dout if need[1] else None), dweight, dgamma, None
+
+
+# ----------------------------------------------------------------------------------------------
+# attention without a stored probability matrix: the backward pass computes the probabilities again
+# ----------------------------------------------------------------------------------------------
+_ATTENTION_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _on_device(t: torch.Tensor):
+    """context: the operators launch on the device that holds their tensors, whichever is current"""
+    return torch.cuda.device(t.device) if t.is_cuda and t.get_device() != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _rows_readable(t):
+    """the tensor itself if the kernels can address its rows (last dimension contiguous), else a contiguous copy"""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides3(t):
+    return t.stride(0), t.stride(1), t.stride(2)
+
+
+def _check_index_vector(name, t, B, like):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (B,):
+        raise ValueError("attention: %s must be an int32 or int64 tensor of shape [%d]" % (name, B))
+    if t.device != like.device:
+        raise ValueError("attention: %s is on %s, q on %s" % (name, t.device, like.device))
+    return t.to(torch.int32).contiguous()
+
+
+class AttentionFn(Function):
+    """Forward: output and log-sum-exp only (icg_attention_fwd).  Backward: the probabilities again, tile by tile (icg_attention_bwd);
+    fixed summation order, no atomics."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, k_lens, q_start, scale, causal):
+        B, Lq, H, d = q.shape
+        Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
+        dt = _ATTENTION_DTYPES[q.dtype]
+        q, k, v = _rows_readable(q), _rows_readable(k), _rows_readable(v)
+        o = torch.empty(B, Lq, H, dv, device=q.device, dtype=q.dtype)
+        lse = torch.empty(B, H, Lq, device=q.device, dtype=torch.float32)
+        if o.numel() == 0 or Lk == 0:
+            o.zero_()
+            lse.fill_(float("-inf"))
+        else:
+            with _on_device(q):
+                nb = L.query("icg_attention_fwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, dt)
+                L.call("icg_attention_fwd", q, k, v, k_lens, q_start, o, lse, B, Lq, Lk, H, Hk, d, dv, *_strides3(q), *_strides3(k), *_strides3(v),
+                       scale, int(causal), dt, _bytes(nb, q.device) if nb else None, nb)
+        ctx.scale, ctx.causal = scale, causal
+        ctx.save_for_backward(q, k, v, o, lse, k_lens, q_start)
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, dlse=None):
+        q, k, v, o, lse, k_lens, q_start = ctx.saved_tensors
+        B, Lq, H, d = q.shape
+        Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
+        dt = _ATTENTION_DTYPES[q.dtype]
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        dk, dv_ = torch.empty(k.shape, device=q.device, dtype=q.dtype), torch.empty(v.shape, device=q.device, dtype=q.dtype)
+        if o.numel() == 0 or Lk == 0:
+            return dq.zero_(), dk.zero_(), dv_.zero_(), None, None, None, None
+        do = _rows_readable(do)
+        with _on_device(q):
+            nb = L.query("icg_attention_bwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, dt)
+            L.call("icg_attention_bwd", q, k, v, o, do, lse, k_lens, q_start, dq, dk, dv_, B, Lq, Lk, H, Hk, d, dv, *_strides3(q), *_strides3(k),
+                   *_strides3(v), *_strides3(do), ctx.scale, int(ctx.causal), dt, _bytes(nb, q.device), nb)
+        return dq, dk, dv_, None, None, None, None
+
+
+def attention(q, k, v, *, scale=None, causal=False, k_lens=None, q_start=None, return_lse=False):
+    """softmax(scale q k^T) v per head, with the probabilities never in memory: o [B, Lq, H, dv] (and, with `return_lse`, the log of the
+    softmax sums [B, H, Lq], fp32, without gradient).  Differentiable once in q, k and v.
+
+    q [B, Lq, H, d], k [B, Lk, Hk, d], v [B, Lk, Hk, dv]: fp32, fp16 or bf16, any strides; H a multiple of Hk (heads h with the same
+    h // (H // Hk) share a key head); d, dv <= 128, or d <= 64 and dv <= 256.
+    scale      > 0, default 1 / sqrt(d)
+    k_lens     [B]: sequence b has its first k_lens[b] keys only (held to 0 .. Lk); what lies behind them is never read
+    causal     query i of sequence b sees keys up to q_start[b] + i
+    q_start    [B], default Lk - Lq: the position of the sequence's first query among the keys (used when causal)
+    A query that sees no key gets zeros, -inf and no gradient.  One or few queries (a token at a time against a cache) take a kernel that
+    splits the keys over the chip."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 4:
+            raise ValueError("attention: %s must be a 4-D tensor [batch, position, head, element]" % name)
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError("attention: q, k and v must have one type and device (q %s on %s, %s %s on %s)" % (q.dtype, q.device, name, t.dtype, t.device))
+    if q.dtype not in _ATTENTION_DTYPES:
+        raise ValueError("attention: fp32, fp16 or bf16, not %s" % q.dtype)
+    B, Lq, H, d = q.shape
+    Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
+    if k.shape[0] != B or v.shape[0] != B or v.shape[1] != Lk or v.shape[2] != Hk or k.shape[3] != d:
+        raise ValueError("attention: shapes do not fit: q %s, k %s, v %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if Hk == 0 or H % Hk != 0:
+        raise ValueError("attention: %d query heads over %d key heads" % (H, Hk))
+    if d == 0 or dv == 0:
+        raise ValueError("attention: heads of no elements")
+    scale = float(d) ** -0.5 if scale is None else float(scale)
+    if not (0.0 < scale < float("inf")):
+        raise ValueError("attention: scale must be positive and finite, not %r" % scale)
+    k_lens, q_start = _check_index_vector("k_lens", k_lens, B, q), _check_index_vector("q_start", q_start, B, q)
+    if B * Lq * Lk and not L.query("icg_attention_applies", B, Lq, Lk, H, Hk, d, dv, _ATTENTION_DTYPES[q.dtype]):
+        raise ValueError("attention: not served: B %d, Lq %d, Lk %d, H %d, d %d, dv %d (d, dv <= 128, or d <= 64 and dv <= 256)" % (B, Lq, Lk, H, d, dv))
+    _require_gpu(q)
+    o, lse = AttentionFn.apply(q, k, v, k_lens, q_start, scale, bool(causal))
+    return (o, lse) if return_lse else o
 
 
 def gemm(a, b, c, m, n, k, trans_a: bool, trans_b: bool, alpha=1.0):

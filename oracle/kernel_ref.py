@@ -1528,6 +1528,53 @@ def nan_to_num_multi_ref(tensors, nan=0.0, posinf=None, neginf=None):
             torch.nan_to_num(t, nan=nan, posinf=posinf, neginf=neginf, out=t)
 
 
+def icg_attention_applies(B, Lq, Lk, H, Hk, d, dv, dtype):
+    return int(min(B, Lq, Lk, H, Hk, d, dv) > 0 and H % Hk == 0 and dtype in (0, 1, 2) and ((d <= 128 and dv <= 128) or (d <= 64 and dv <= 256)))
+
+
+def icg_attention_fwd_workspace_bytes(*a):
+    return 0
+
+
+def icg_attention_bwd_workspace_bytes(B, Lq, Lk, H, Hk, d, dv, dtype):
+    return 12 * B * H * Lq
+
+
+def _attention_probabilities(q, k, v, k_lens, q_start, Hk, scale, causal):
+    """-> q, k, v as fp32 [B, H, L, e] (key heads repeated, nothing behind k_lens), p and lse"""
+    B, Lq, H, _ = q.shape
+    Lk = k.shape[1]
+    j, i = torch.arange(Lk).view(1, 1, 1, -1), torch.arange(Lq).view(1, 1, -1, 1)
+    keys = (torch.full((B,), Lk) if k_lens is None else k_lens.long().clamp(0, Lk)).view(B, 1, 1, 1)
+    m = j < keys
+    if causal:
+        m = m & (j <= (torch.full((B,), Lk - Lq) if q_start is None else q_start.long()).view(B, 1, 1, 1) + i)
+    Q, K, V = (t.detach().float().transpose(1, 2) for t in (q, k, v))
+    gone = (j >= keys).transpose(-1, -2)
+    K, V = (t.masked_fill(gone, 0.0).repeat_interleave(H // Hk, 1) for t in (K, V))
+    s = (Q @ K.transpose(-1, -2) * scale).masked_fill(~m, -math.inf)
+    lse = torch.logsumexp(s, -1)
+    return Q, K, V, torch.exp(s - lse.unsqueeze(-1).nan_to_num(neginf=0.0)), lse
+
+
+def icg_attention_fwd(q, k, v, k_lens, q_start, o, lse, B, Lq, Lk, H, Hk, d, dv, *rest):
+    scale, causal = rest[9], rest[10]
+    _, _, V, p, l = _attention_probabilities(q, k, v, k_lens, q_start, Hk, scale, causal)
+    o.copy_((p @ V).transpose(1, 2))
+    lse.copy_(l)
+
+
+def icg_attention_bwd(q, k, v, o, dout, lse, k_lens, q_start, dq, dk, dv_out, B, Lq, Lk, H, Hk, d, dv, *rest):
+    scale, causal = rest[12], rest[13]
+    Q, K, V, p, _ = _attention_probabilities(q, k, v, k_lens, q_start, Hk, scale, causal)
+    dO = dout.detach().float().transpose(1, 2)
+    ds = p * (dO @ V.transpose(-1, -2) - (dO * o.float().transpose(1, 2)).sum(-1, keepdim=True)) * scale
+    shared = lambda t: t.reshape(B, Hk, H // Hk, Lk, -1).sum(2).transpose(1, 2)
+    dq.copy_((ds @ K).transpose(1, 2))
+    dk.copy_(shared(ds.transpose(-1, -2) @ Q))
+    dv_out.copy_(shared(p.transpose(-1, -2) @ dO))
+
+
 def install(monkeypatch):
     """Route ic_gan_amd._lib.call / query to this module (CPU host-logic tests only)."""
     import ic_gan_amd._lib as L
