@@ -1320,7 +1320,7 @@ class AttnOutFn(Function):
 # ----------------------------------------------------------------------------------------------
 # attention without a stored probability matrix: the backward pass computes the probabilities again
 # ----------------------------------------------------------------------------------------------
-_ATTENTION_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 def _on_device(t: torch.Tensor):
@@ -1355,7 +1355,7 @@ class AttentionFn(Function):
     def forward(ctx, q, k, v, k_lens, q_start, scale, causal):
         B, Lq, H, d = q.shape
         Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
-        dt = _ATTENTION_DTYPES[q.dtype]
+        dt = _DTYPE_CODES[q.dtype]
         q, k, v = _rows_readable(q), _rows_readable(k), _rows_readable(v)
         o = torch.empty(B, Lq, H, dv, device=q.device, dtype=q.dtype)
         lse = torch.empty(B, H, Lq, device=q.device, dtype=torch.float32)
@@ -1378,7 +1378,7 @@ class AttentionFn(Function):
         q, k, v, o, lse, k_lens, q_start = ctx.saved_tensors
         B, Lq, H, d = q.shape
         Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
-        dt = _ATTENTION_DTYPES[q.dtype]
+        dt = _DTYPE_CODES[q.dtype]
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         dk, dv_ = torch.empty(k.shape, device=q.device, dtype=q.dtype), torch.empty(v.shape, device=q.device, dtype=q.dtype)
         if o.numel() == 0 or Lk == 0:
@@ -1408,7 +1408,7 @@ def attention(q, k, v, *, scale=None, causal=False, k_lens=None, q_start=None, r
             raise ValueError("attention: %s must be a 4-D tensor [batch, position, head, element]" % name)
         if t.dtype != q.dtype or t.device != q.device:
             raise ValueError("attention: q, k and v must have one type and device (q %s on %s, %s %s on %s)" % (q.dtype, q.device, name, t.dtype, t.device))
-    if q.dtype not in _ATTENTION_DTYPES:
+    if q.dtype not in _DTYPE_CODES:
         raise ValueError("attention: fp32, fp16 or bf16, not %s" % q.dtype)
     B, Lq, H, d = q.shape
     Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
@@ -1422,11 +1422,149 @@ def attention(q, k, v, *, scale=None, causal=False, k_lens=None, q_start=None, r
     if not (0.0 < scale < float("inf")):
         raise ValueError("attention: scale must be positive and finite, not %r" % scale)
     k_lens, q_start = _check_index_vector("k_lens", k_lens, B, q), _check_index_vector("q_start", q_start, B, q)
-    if B * Lq * Lk and not L.query("icg_attention_applies", B, Lq, Lk, H, Hk, d, dv, _ATTENTION_DTYPES[q.dtype]):
+    if B * Lq * Lk and not L.query("icg_attention_applies", B, Lq, Lk, H, Hk, d, dv, _DTYPE_CODES[q.dtype]):
         raise ValueError("attention: not served: B %d, Lq %d, Lk %d, H %d, d %d, dv %d (d, dv <= 128, or d <= 64 and dv <= 256)" % (B, Lq, Lk, H, d, dv))
     _require_gpu(q)
     o, lse = AttentionFn.apply(q, k, v, k_lens, q_start, scale, bool(causal))
     return (o, lse) if return_lse else o
+
+
+# ----------------------------------------------------------------------------------------------
+# group norm with an activation, channels last
+# ----------------------------------------------------------------------------------------------
+_ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
+
+
+class GroupNormActFn(Function):
+    @staticmethod
+    def forward(ctx, x, gain, bias, groups, gain_offset, eps, act):
+        x = x.contiguous(memory_format=torch.channels_last)
+        B, C, H, W = x.shape
+        affine = gain if gain is not None else bias
+        per_sample = int(affine is not None and affine.dim() == 2)
+        dt = _DTYPE_CODES[x.dtype]
+        y = torch.empty_like(x)
+        mean, rstd = _f32(B * groups, x.device), _f32(B * groups, x.device)
+        ctx.meta = (groups, per_sample, gain_offset, eps, act, dt)
+        if x.numel():
+            with _on_device(x):
+                nb = L.query("icg_groupnorm_fwd_workspace_bytes", B, H * W, C, groups, dt)
+                L.call("icg_groupnorm_act_fwd", x, gain, bias, y, mean, rstd, B, H * W, C, groups, per_sample, gain_offset, eps, act, dt,
+                       _bytes(nb, x.device) if nb else None, nb)
+        ctx.save_for_backward(x, gain, bias, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, gain, bias, mean, rstd = ctx.saved_tensors
+        groups, per_sample, gain_offset, eps, act, dt = ctx.meta
+        B, C, H, W = x.shape
+        dy = dy.contiguous(memory_format=torch.channels_last)
+        dx = torch.empty_like(x)
+        dgain = dbias = None
+        if gain is not None or bias is not None:
+            shape = (B, C) if per_sample else (C,)
+            dgain, dbias = (torch.empty(shape, device=x.device, dtype=torch.float32) for _ in range(2))
+        if x.numel():
+            with _on_device(x):
+                nb = L.query("icg_groupnorm_bwd_workspace_bytes", B, H * W, C, groups, dt)
+                L.call("icg_groupnorm_act_bwd", x, dy, gain, bias, mean, rstd, dx, dgain, dbias, B, H * W, C, groups, per_sample, gain_offset, eps,
+                       act, dt, _bytes(nb, x.device), nb)
+        elif dgain is not None:
+            dgain.zero_(), dbias.zero_()
+        return dx, (dgain if gain is not None else None), (dbias if bias is not None else None), None, None, None, None
+
+
+def group_norm_act(x, groups, gain=None, bias=None, *, eps=1e-5, act="none", gain_offset=0.0):
+    """act(group_norm(x) * (gain_offset + gain) + bias) in the layout of x [B, C, H, W] (channels last; another layout is converted).
+
+    x: fp32, fp16 or bf16; statistics and arithmetic in fp32, one rounding.  groups divides C.  gain, bias: [C], or [B, C] for a
+    conditional norm (both of one shape; None: 1 and 0).  act: "none", "relu" or "silu".  Differentiable once in x, gain and bias; nothing but
+    x and the groups' mean and 1 / deviation is kept for the gradient."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 4:
+        raise ValueError("group_norm_act: x must be a 4-D activation [batch, channel, height, width]")
+    if x.dtype not in _DTYPE_CODES:
+        raise ValueError("group_norm_act: fp32, fp16 or bf16, not %s" % x.dtype)
+    B, C = x.shape[:2]
+    if not isinstance(groups, int) or groups < 1 or C % groups != 0:
+        raise ValueError("group_norm_act: %r groups over %d channels" % (groups, C))
+    if act not in _ACTIVATIONS:
+        raise ValueError("group_norm_act: act must be one of %s, not %r" % (sorted(_ACTIVATIONS), act))
+    if not (0.0 <= float(eps) < float("inf")):
+        raise ValueError("group_norm_act: eps must be finite and not negative, not %r" % eps)
+    for name, t in (("gain", gain), ("bias", bias)):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or tuple(t.shape) not in ((C,), (B, C)) or not t.is_floating_point():
+            raise ValueError("group_norm_act: %s must be a floating-point tensor of shape [%d] or [%d, %d]" % (name, C, B, C))
+        if t.device != x.device:
+            raise ValueError("group_norm_act: %s is on %s, x on %s" % (name, t.device, x.device))
+    if gain is not None and bias is not None and gain.shape != bias.shape:
+        raise ValueError("group_norm_act: gain %s and bias %s differ in shape" % (tuple(gain.shape), tuple(bias.shape)))
+    _require_gpu(x)
+    gain, bias = (t if t is None else t.float().contiguous() for t in (gain, bias))
+    return GroupNormActFn.apply(x, gain, bias, groups, float(gain_offset), float(eps), _ACTIVATIONS[act])
+
+
+# ----------------------------------------------------------------------------------------------
+# embedding lookup with scaling; gradient by sorted tokens
+# ----------------------------------------------------------------------------------------------
+def embedding_backward(idx, dout, V, scale=1.0, padding_idx=None):
+    """[V, D]: scale times the sum of dout's rows over the positions of each token, in the order of the positions (icg_embedding_bwd)."""
+    D = dout.shape[-1]
+    flat, d2 = idx.reshape(-1).contiguous(), dout.reshape(-1, D).contiguous()
+    dw = torch.empty(V, D, device=dout.device, dtype=dout.dtype)
+    if flat.numel() == 0 or dw.numel() == 0:
+        return dw.zero_()
+    dt = _DTYPE_CODES[dout.dtype]
+    with _on_device(dout):
+        nb = L.query("icg_embedding_bwd_workspace_bytes", flat.numel(), V, D, dt)
+        L.call("icg_embedding_bwd", flat, d2, dw, flat.numel(), V, D, scale, -1 if padding_idx is None else padding_idx, int(flat.dtype == torch.int64),
+               dt, _bytes(nb, dout.device) if nb else None, nb)
+    return dw
+
+
+class EmbeddingFn(Function):
+    @staticmethod
+    def forward(ctx, idx, weight, scale, padding_idx):
+        w, flat = weight.contiguous(), idx.contiguous()
+        V, D = w.shape
+        out = torch.empty(*idx.shape, D, device=w.device, dtype=w.dtype)
+        if out.numel():
+            with _on_device(w):
+                L.call("icg_embedding_fwd", flat, w, out, flat.numel(), V, D, scale, int(flat.dtype == torch.int64), _DTYPE_CODES[w.dtype])
+        ctx.meta = (V, scale, padding_idx)
+        ctx.save_for_backward(flat)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        (flat,) = ctx.saved_tensors
+        V, scale, padding_idx = ctx.meta
+        return None, embedding_backward(flat, dout, V, scale, padding_idx), None, None
+
+
+def embedding(idx, weight, *, scale=1.0, padding_idx=None):
+    """scale * weight[idx]: idx int64 or int32 of any shape, weight [V, D] fp32, fp16 or bf16 -> [*idx.shape, D].  The gradient of the table is
+    dense, summed in fp32 in the order of the positions (the same bits on every run) and rounded once; rows whose token does not occur are zero,
+    and so is `padding_idx`'s.  A token outside the table gives a row of NaN (nothing is read) and no gradient."""
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.dtype not in _DTYPE_CODES:
+        raise ValueError("embedding: weight must be a 2-D fp32, fp16 or bf16 tensor")
+    if not isinstance(idx, torch.Tensor) or idx.dtype not in (torch.int32, torch.int64):
+        raise ValueError("embedding: idx must be an int32 or int64 tensor")
+    if idx.device != weight.device:
+        raise ValueError("embedding: idx is on %s, weight on %s" % (idx.device, weight.device))
+    V, D = weight.shape
+    if V == 0 or D == 0 or D >= 1 << 24 or max(V, idx.numel()) >= 0x7fffff00:
+        raise ValueError("embedding: not served: table [%d, %d], %d tokens" % (V, D, idx.numel()))
+    if not abs(float(scale)) < float("inf"):
+        raise ValueError("embedding: scale must be finite, not %r" % scale)
+    if padding_idx is not None and not 0 <= padding_idx < V:
+        raise ValueError("embedding: padding_idx %r outside the table of %d rows" % (padding_idx, V))
+    _require_gpu(weight)
+    return EmbeddingFn.apply(idx, weight, float(scale), padding_idx)
 
 
 def gemm(a, b, c, m, n, k, trans_a: bool, trans_b: bool, alpha=1.0):

@@ -806,6 +806,27 @@ int icg_attention_bwd(const void* q, const void* k, const void* v, const void* o
                       int64_t do_sb, int64_t do_sl, int64_t do_sh, float scale, int causal, int dtype, void* workspace, size_t workspace_bytes,
                       void* stream);
 
+/* ---- group norm with an activation, channels last (csrc/groupnorm.hip; beside the icg_bn_* entry points) ----
+ *   y = act(xh (g0 + gain) + bias),  xh = (x - m) / sqrt(v + eps),  m, v over HW and the C / G channels of a group, per sample
+ * x, y, dy, dx [B][HW][C] of dtype 0 / 1 / 2 = fp32 / fp16 / bf16; gain, bias (NULL: 1 and 0), dgain, dbias fp32 [C], or [B][C] with per_sample;
+ * act 0 none, 1 ReLU, 2 SiLU.  mean, rstd [B][G] fp32 leave the forward and enter the gradient, which forms act' again from x.  dgain and
+ * dbias may both be NULL.  One launch where a group's slab fits a workgroup's registers, three (x read twice) elsewhere. */
+size_t icg_groupnorm_fwd_workspace_bytes(int B, int64_t HW, int C, int G, int dtype);
+int icg_groupnorm_act_fwd(const void* x, const float* gain, const float* bias, void* y, float* mean, float* rstd, int B, int64_t HW, int C, int G,
+                          int per_sample, float gain_offset, float eps, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t icg_groupnorm_bwd_workspace_bytes(int B, int64_t HW, int C, int G, int dtype);
+int icg_groupnorm_act_bwd(const void* x, const void* dy, const float* gain, const float* bias, const float* mean, const float* rstd, void* dx,
+                          float* dgain, float* dbias, int B, int64_t HW, int C, int G, int per_sample, float gain_offset, float eps, int act,
+                          int dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* ---- embedding lookup with scaling and its dense gradient by sorted tokens (csrc/embedding.hip) ----
+ *   out[i] = scale W[idx[i]];   dweight[v] = scale sum_{i: idx[i] = v} dout[i]  (in the order of i, fp32 sums; rows without tokens are zero)
+ * idx [n] int64 (idx64) or int32, weight / dweight [V][D], out / dout [n][D] of dtype 0 / 1 / 2.  A token outside 0 .. V - 1 gives a row of
+ * NaN and no gradient; the token `pad` (-1: none) gets no gradient. */
+int icg_embedding_fwd(const void* idx, const void* weight, void* out, int64_t n, int64_t V, int64_t D, float scale, int idx64, int dtype, void* stream);
+size_t icg_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D, int dtype);
+int icg_embedding_bwd(const void* idx, const void* dout, void* dweight, int64_t n, int64_t V, int64_t D, float scale, int64_t pad, int idx64, int dtype,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

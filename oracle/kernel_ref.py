@@ -1575,6 +1575,66 @@ def icg_attention_bwd(q, k, v, o, dout, lse, k_lens, q_start, dq, dk, dv_out, B,
     dv_out.copy_(shared(p.transpose(-1, -2) @ dO))
 
 
+def icg_groupnorm_fwd_workspace_bytes(*a):
+    return 0
+
+
+def icg_groupnorm_bwd_workspace_bytes(B, HW, C, G, dtype):
+    return 8 * B * C
+
+
+def _groupnorm_parts(x, gain, bias, B, HW, C, G, per_sample, g0, mean, rstd, act):
+    """-> xh, g0 + gain, z, act'(z) as fp32 [B, HW, C]"""
+    xs = mem(x).view(B, HW, C).float()
+    each = lambda t: t.view(B, 1, G).repeat_interleave(C // G, 2)
+    xh = (xs - each(mean)) * each(rstd)
+    row = lambda t, one: torch.full((1, 1, C), one) if t is None else mem(t).view(B if per_sample else 1, 1, C)
+    g = row(gain, 1.0) + (g0 if gain is not None else 0.0)
+    z = xh * g + row(bias, 0.0)
+    s = torch.sigmoid(z)
+    return xh, g, z, {0: torch.ones_like(z), 1: (z > 0).float(), 2: s * (1 + z * (1 - s))}[act]
+
+
+def icg_groupnorm_act_fwd(x, gain, bias, y, mean, rstd, B, HW, C, G, per_sample, gain_offset, eps, act, dtype, workspace, workspace_bytes):
+    var, mu = torch.var_mean(mem(x).view(B, HW, G, C // G).double(), (1, 3), correction=0)
+    mean.copy_(mu.reshape(-1))
+    rstd.copy_((var + eps).rsqrt().reshape(-1))
+    _, _, z, _ = _groupnorm_parts(x, gain, bias, B, HW, C, G, per_sample, gain_offset, mean, rstd, act)
+    out = z if act == 0 else F.relu(z) if act == 1 else F.silu(z)
+    _nhwc(y, B, 1, HW, C).copy_(out.view(B, 1, HW, C)) if y.is_contiguous() else y.copy_(out.view(B, y.shape[2], y.shape[3], C).permute(0, 3, 1, 2))
+
+
+def icg_groupnorm_act_bwd(x, dy, gain, bias, mean, rstd, dx, dgain, dbias, B, HW, C, G, per_sample, gain_offset, eps, act, dtype, workspace,
+                          workspace_bytes):
+    xh, g, z, da = _groupnorm_parts(x, gain, bias, B, HW, C, G, per_sample, gain_offset, mean, rstd, act)
+    dz = mem(dy).view(B, HW, C).float() * da
+    if dgain is not None:
+        sums = [(dz * xh).sum(1), dz.sum(1)]
+        dgain.copy_(sums[0] if per_sample else sums[0].sum(0))
+        dbias.copy_(sums[1] if per_sample else sums[1].sum(0))
+    dn = dz * g
+    mean_of = lambda t: t.view(B, HW, G, C // G).mean((1, 3), keepdim=True).expand(B, HW, G, C // G).reshape(B, HW, C)
+    out = (dn - mean_of(dn) - xh * mean_of(dn * xh)) * rstd.view(B, 1, G).repeat_interleave(C // G, 2)
+    dx.copy_(out.view(B, dx.shape[2], dx.shape[3], C).permute(0, 3, 1, 2))
+
+
+def icg_embedding_fwd(idx, weight, out, n, V, D, scale, idx64, dtype):
+    t = idx.reshape(-1).long()
+    rows = weight[t.clamp(0, V - 1)].float() * scale
+    out.copy_(rows.masked_fill(((t < 0) | (t >= V)).view(-1, 1), float("nan")).view(out.shape))
+
+
+def icg_embedding_bwd_workspace_bytes(n, V, D, dtype):
+    return 16 if n > 1024 else 0
+
+
+def icg_embedding_bwd(idx, dout, dweight, n, V, D, scale, pad, idx64, dtype, workspace, workspace_bytes):
+    t = idx.reshape(-1).long()
+    ok = (t >= 0) & (t < V) & (t != pad)
+    acc = torch.zeros(V, D).index_add_(0, t[ok], dout.reshape(n, D)[ok].float())
+    dweight.copy_(acc * scale)
+
+
 def install(monkeypatch):
     """Route ic_gan_amd._lib.call / query to this module (CPU host-logic tests only)."""
     import ic_gan_amd._lib as L
