@@ -106,7 +106,9 @@ class Generator(nn.Module):
                  G_B2=0.999, adam_eps=1e-8, BN_eps=1e-5, SN_eps=1e-12, G_mixed_precision=False, G_fp16=False,
                  G_init="ortho", skip_init=False, no_optim=False, G_param="SN", norm_style="bn", class_cond=True,
                  embedded_optimizer=True, instance_cond=False, G_shared_feat=True, shared_dim_feat=2048,
-                 sync_bn=False, **kwargs):
+                 sync_bn=False, attn_recompute=False, sorted_embedding=False, **kwargs):
+        """Beside the reference's arguments: sync_bn; attn_recompute (layers.Attention: no stored probabilities); sorted_embedding
+        (layers.Embedding for the class embedding); norm_style 'gn' / 'gn_<groups>' (conditional group norm in the blocks)."""
         super().__init__()
         if G_param != "SN":
             raise NotImplementedError("ic_gan_amd.Generator: G_param='SN' only (every shipped config)")
@@ -136,7 +138,7 @@ class Generator(nn.Module):
         sn_kw = dict(num_svs=num_G_SVs, num_itrs=num_G_SV_itrs, eps=self.SN_eps)
         self.which_conv = functools.partial(layers.SNConv2d, kernel_size=3, padding=1, **sn_kw)
         self.which_linear = functools.partial(layers.SNLinear, **sn_kw)
-        self.which_embedding = nn.Embedding   # G's class embedding is not spectrally normalised (BigGAN.py:205-207)
+        self.which_embedding = layers.Embedding if sorted_embedding else nn.Embedding   # G's class embedding is not spectrally normalised (BigGAN.py:205-207)
         bn_linear = functools.partial(self.which_linear, bias=False) if self.G_shared else self.which_embedding
         cond_width = self.z_chunk_size if (class_cond or instance_cond) else self.n_classes
         if class_cond:
@@ -159,7 +161,7 @@ class Generator(nn.Module):
                                              if self.arch["upsample"][i] else None))]
             if self.arch["attention"][self.arch["resolution"][i]]:
                 print("Adding attention layer in G at resolution %d" % self.arch["resolution"][i])
-                stage.append(layers.Attention(self.arch["out_channels"][i], self.which_conv))
+                stage.append(layers.Attention(self.arch["out_channels"][i], self.which_conv, recompute=attn_recompute))
             stages.append(nn.ModuleList(stage))
         self.blocks = nn.ModuleList(stages)
         self.output_layer = _OutputLayer(
@@ -223,7 +225,7 @@ class Discriminator(nn.Module):
                  num_D_SVs=1, num_D_SV_itrs=1, D_activation=nn.ReLU(inplace=False), D_lr=2e-4, D_B1=0.0, D_B2=0.999,
                  adam_eps=1e-8, SN_eps=1e-12, output_dim=1, D_mixed_precision=False, D_fp16=False, D_init="ortho",
                  skip_init=False, D_param="SN", class_cond=True, embedded_optimizer=True, instance_cond=False,
-                 instance_sz=2048, **kwargs):
+                 instance_sz=2048, attn_recompute=False, **kwargs):
         super().__init__()
         if D_param != "SN":
             raise NotImplementedError("ic_gan_amd.Discriminator: D_param='SN' only")
@@ -248,7 +250,7 @@ class Discriminator(nn.Module):
                                    downsample=(nn.AvgPool2d(2) if self.arch["downsample"][i] else None))]
             if self.arch["attention"][self.arch["resolution"][i]]:
                 print("Adding attention layer in D at resolution %d" % self.arch["resolution"][i])
-                stage.append(layers.Attention(self.arch["out_channels"][i], self.which_conv))
+                stage.append(layers.Attention(self.arch["out_channels"][i], self.which_conv, recompute=attn_recompute))
             stages.append(nn.ModuleList(stage))
         self.blocks = nn.ModuleList(stages)
         top = self.arch["out_channels"][-1]

@@ -95,12 +95,17 @@ class GBlock(nn.Module):
     def forward(self, x, y):
         up = bool(self.upsample)
         (g1, b1), (g2, b2), (g3, b3), (g4, b4) = (_cond(m, y) for m in (self.bn1, self.bn2, self.bn3, self.bn4))
-        h = self.conv1(x, relu=True, bn=self.bn1.bn_opt(), gain=g1, beta=b1)
-        h = self.conv2(h, relu=True, upsample=up, bn=self.bn2.bn_opt(), gain=g2, beta=b2)
-        h = self.conv3(h, relu=True, bn=self.bn3.bn_opt(), gain=g3, beta=b3)
         skip = x
         if self.in_channels != self.out_channels:          # drop channels (BigGANdeep.py:73-74)
             skip = x[:, : self.out_channels].contiguous(memory_format=torch.channels_last)
+        if isinstance(self.bn1, layers.ccbn) and self.bn1.groups is not None:      # group norm + ReLU are their own pass
+            h = self.conv1(self.bn1.act(x, g1, b1))
+            h = self.conv2(self.bn2.act(h, g2, b2), upsample=up)
+            h = self.conv3(self.bn3.act(h, g3, b3))
+            return self.conv4(self.bn4.act(h, g4, b4), residual=skip, res_up=up)
+        h = self.conv1(x, relu=True, bn=self.bn1.bn_opt(), gain=g1, beta=b1)
+        h = self.conv2(h, relu=True, upsample=up, bn=self.bn2.bn_opt(), gain=g2, beta=b2)
+        h = self.conv3(h, relu=True, bn=self.bn3.bn_opt(), gain=g3, beta=b3)
         return self.conv4(h, relu=True, bn=self.bn4.bn_opt(), gain=g4, beta=b4, residual=skip, res_up=up)
 
 
@@ -152,7 +157,8 @@ class Generator(nn.Module):
                  cross_replica=False, mybn=False, G_activation=nn.ReLU(inplace=False), G_lr=5e-5, G_B1=0.0, G_B2=0.999,
                  adam_eps=1e-8, BN_eps=1e-5, SN_eps=1e-12, G_mixed_precision=False, G_fp16=False, G_init="ortho",
                  skip_init=False, no_optim=False, G_param="SN", norm_style="bn", sync_bn=False, class_cond=True,
-                 instance_cond=False, G_shared_feat=True, shared_dim_feat=2048, **kwargs):
+                 instance_cond=False, G_shared_feat=True, shared_dim_feat=2048, attn_recompute=False, sorted_embedding=False,
+                 **kwargs):
         super().__init__()
         if G_param != "SN":
             raise NotImplementedError("ic_gan_amd.BigGANdeep.Generator: G_param='SN' only")
@@ -177,7 +183,7 @@ class Generator(nn.Module):
         sn_kw = dict(num_svs=num_G_SVs, num_itrs=num_G_SV_itrs, eps=self.SN_eps)
         self.which_conv = functools.partial(layers.SNConv2d, kernel_size=3, padding=1, **sn_kw)
         self.which_linear = functools.partial(layers.SNLinear, **sn_kw)
-        self.which_embedding = nn.Embedding
+        self.which_embedding = layers.Embedding if sorted_embedding else nn.Embedding
         bn_linear = functools.partial(self.which_linear, bias=False) if self.G_shared else self.which_embedding
         # width of the conditioning vector y: class embedding (++ instance embedding, BigGAN.py:350-358 by analogy)
         self.cond_dim = (self.shared_dim if class_cond else 0) + self.shared_dim_feat
@@ -206,7 +212,7 @@ class Generator(nn.Module):
                      for g in range(self.G_depth)]
             if self.arch["attention"][self.arch["resolution"][i]]:
                 print("Adding attention layer in G at resolution %d" % self.arch["resolution"][i])
-                group[-1].append(layers.Attention(self.arch["out_channels"][i], self.which_conv))
+                group[-1].append(layers.Attention(self.arch["out_channels"][i], self.which_conv, recompute=attn_recompute))
             stages.extend(nn.ModuleList(b) for b in group)
         self.blocks = nn.ModuleList(stages)
         self.output_layer = _OutputLayer(
@@ -259,7 +265,8 @@ class Discriminator(nn.Module):
     def __init__(self, D_ch=64, D_wide=True, D_depth=2, resolution=128, D_kernel_size=3, D_attn="64", n_classes=1000,
                  num_D_SVs=1, num_D_SV_itrs=1, D_activation=nn.ReLU(inplace=False), D_lr=2e-4, D_B1=0.0, D_B2=0.999,
                  adam_eps=1e-8, SN_eps=1e-12, output_dim=1, D_mixed_precision=False, D_fp16=False, D_init="ortho",
-                 skip_init=False, D_param="SN", class_cond=True, instance_cond=False, instance_sz=2048, **kwargs):
+                 skip_init=False, D_param="SN", class_cond=True, instance_cond=False, instance_sz=2048, attn_recompute=False,
+                 **kwargs):
         super().__init__()
         if D_param != "SN":
             raise NotImplementedError("ic_gan_amd.BigGANdeep.Discriminator: D_param='SN' only")
@@ -284,7 +291,7 @@ class Discriminator(nn.Module):
                      for d in range(self.D_depth)]
             if self.arch["attention"][self.arch["resolution"][i]]:
                 print("Adding attention layer in D at resolution %d" % self.arch["resolution"][i])
-                stage.append(layers.Attention(self.arch["out_channels"][i], self.which_conv))
+                stage.append(layers.Attention(self.arch["out_channels"][i], self.which_conv, recompute=attn_recompute))
             stages.append(nn.ModuleList(stage))
         self.blocks = nn.ModuleList(stages)
         top = self.arch["out_channels"][-1]

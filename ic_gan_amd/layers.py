@@ -14,7 +14,7 @@ sequence of fused HIP kernels (``ic_gan_amd.ops``):
 
 Unsupported reference options (never used by a shipped config) raise NotImplementedError instead of
 silently taking another path: num_svs/num_itrs != 1, mybn, the reference's `cross_replica` nn.BatchNorm2d
-variant (use `sync_bn=True`: cross-replica statistics over RCCL with the same buffers), norm_style != 'bn'.
+variant (use `sync_bn=True`: cross-replica statistics over RCCL with the same buffers), norm_style other than 'bn' and 'gn'.
 """
 from __future__ import annotations
 
@@ -231,6 +231,20 @@ class SNEmbedding(nn.Embedding, SN):
         return ops.SNEmbeddingFn.apply(x, self.weight if st.handle is None else st.handle, st)
 
 
+class Embedding(nn.Embedding):
+    """nn.Embedding (same parameter and arguments) on ops.embedding: the lookup times `scale`, the table's gradient summed in the order of the
+    positions (deterministic)."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0, **kwargs):
+        super().__init__(num_embeddings, embedding_dim, padding_idx, **kwargs)
+        if self.max_norm is not None or self.scale_grad_by_freq or self.sparse:
+            raise NotImplementedError("ic_gan_amd.Embedding: max_norm, scale_grad_by_freq and sparse are not implemented")
+        self.scale = float(scale)
+
+    def forward(self, input):
+        return ops.embedding(input, self.weight, scale=self.scale, padding_idx=self.padding_idx)
+
+
 class identity(nn.Module):
     def forward(self, input):
         return input
@@ -239,9 +253,22 @@ class identity(nn.Module):
 # ------------------------------------------------------------------------------------------------
 # Normalisation  (reference layers.py:359-503)
 # ------------------------------------------------------------------------------------------------
+def norm_groups(norm_style):
+    """None for 'bn'; the number of groups for 'gn' (16, the reference's default) and 'gn_<groups>'."""
+    if norm_style == "bn":
+        return None
+    if norm_style == "gn":
+        return 16
+    head, _, count = str(norm_style).partition("_")
+    if head == "gn" and count.isdigit() and int(count) > 0:
+        return int(count)
+    raise NotImplementedError("ic_gan_amd: norm_style 'bn' (all shipped configs), 'gn' or 'gn_<groups>', not %r" % (norm_style,))
+
+
 def _check_bn_variant(cross_replica, mybn, norm_style="bn"):
-    if mybn or norm_style != "bn":
-        raise NotImplementedError("ic_gan_amd: only norm_style='bn' with mybn=False (all shipped configs)")
+    if mybn:
+        raise NotImplementedError("ic_gan_amd: mybn=False only (all shipped configs)")
+    norm_groups(norm_style)
     if cross_replica:
         raise NotImplementedError(
             "the reference's cross_replica=True builds a plain nn.BatchNorm2d (SURVEY F2); use sync_bn=True for "
@@ -251,7 +278,8 @@ def _check_bn_variant(cross_replica, mybn, norm_style="bn"):
 class ccbn(nn.Module):
     """Class / instance-conditional BatchNorm.  The normalise + affine (+ReLU, + upsample) is applied inside the
     next convolution; this module owns the parameters / running statistics and produces the per-sample
-    gain and bias."""
+    gain and bias.  norm_style 'gn': group norm instead (per sample: no running statistics, nothing to exchange between
+    replicas), normalised, scaled and activated by one operator (`act`) in front of the convolution."""
 
     def __init__(self, output_size, input_size, which_linear, eps=1e-5, momentum=0.1, cross_replica=False,
                  mybn=False, norm_style="bn", sync_bn=False):
@@ -262,6 +290,11 @@ class ccbn(nn.Module):
         self.bias = which_linear(input_size, output_size)
         self.eps, self.momentum = eps, momentum
         self.cross_replica, self.mybn, self.norm_style, self.sync_bn = cross_replica, mybn, norm_style, sync_bn
+        self.groups = norm_groups(norm_style)
+        if self.groups is not None:
+            if output_size % self.groups != 0:
+                raise ValueError("norm_style=%r: %d groups over %d channels" % (norm_style, self.groups, output_size))
+            return
         self.register_buffer("stored_mean", torch.zeros(output_size))
         self.register_buffer("stored_var", torch.ones(output_size))
 
@@ -274,8 +307,14 @@ class ccbn(nn.Module):
         return ops.BNOpt(self.stored_mean, self.stored_var, self.eps, 0.1, self.training, 1.0,
                          True if self.sync_bn else None)
 
+    def act(self, x, gain, beta, act="relu"):
+        """norm_style 'gn': act(group norm of x, with the gain and bias that `affine` gave)"""
+        return ops.group_norm_act(x, self.groups, gain, beta, eps=self.eps, act=act, gain_offset=1.0)
+
     def forward(self, x, y):
         gain, beta = self.affine(y)
+        if self.groups is not None:
+            return self.act(x, gain, beta, "none")
         return ops.norm_act(x, self.bn_opt(), gain, beta, relu=False)
 
     def extra_repr(self):
@@ -324,9 +363,12 @@ def _plain_1x1(*convs):
 
 
 class Attention(nn.Module):
-    def __init__(self, ch, which_conv=SNConv2d, name="attention"):
+    """recompute: keep the output and the softmax's log sums for the backward pass instead of the [B, H W, H W / 4] probabilities
+    (ops.attention; 1 GiB less per call at 64 x 64, batch 64)."""
+
+    def __init__(self, ch, which_conv=SNConv2d, name="attention", recompute=False):
         super().__init__()
-        self.ch, self.which_conv = ch, which_conv
+        self.ch, self.which_conv, self.recompute = ch, which_conv, bool(recompute)
         self.theta = which_conv(ch, ch // 8, kernel_size=1, padding=0, bias=False)
         self.phi = which_conv(ch, ch // 8, kernel_size=1, padding=0, bias=False)
         self.g = which_conv(ch, ch // 2, kernel_size=1, padding=0, bias=False)
@@ -348,7 +390,7 @@ class Attention(nn.Module):
             phi, x = self.phi(x, chain=True)
             g, x = self.g(x, chain=True)
             phi, g = ops.MaxPool2Fn.apply(phi), ops.MaxPool2Fn.apply(g)
-        a = ops.AttnCoreFn.apply(theta, phi, g)
+        a = ops.image_attention(theta, phi, g) if self.recompute else ops.AttnCoreFn.apply(theta, phi, g)
         if ops.FUSED_ATTENTION_OUTPUT and _plain_1x1(self.o):
             # gamma folded into the output projection's weight, x added in its epilogue (ops.AttnOutFn).  The weight gradient needs
             # W / sigma in the [Cin][Cout] layout, so that layout is prepared whenever a gradient can be asked for
@@ -383,6 +425,8 @@ class GBlock(nn.Module):
 
     def forward(self, x, y):
         up = bool(self.upsample)
+        if isinstance(self.bn1, ccbn) and self.bn1.groups is not None:
+            return self._forward_group_norm(x, y, up)
         o1, o2 = self.bn1.bn_opt(), self.bn2.bn_opt()
         if ops._sync_enabled(o1):
             return self._forward_sync(x, y, up, o1, o2)
@@ -400,6 +444,17 @@ class GBlock(nn.Module):
             sc = x
         h = self.conv1(x, relu=True, upsample=up, bn=o1, gain=g1, beta=b1)
         return self.conv2(h, relu=True, bn=o2, gain=g2, beta=b2, residual=sc, res_up=up)
+
+    def _forward_group_norm(self, x, y, up):
+        """Group norm needs a sample's statistics before its first value leaves, so it is its own pass (ops.group_norm_act, ReLU inside)
+        and the convolutions read its output."""
+        g1, b1, g2, b2 = ccbn_affine_pair(self.bn1, self.bn2, y)
+        if self.learnable_sc:
+            sc, x = self.conv_sc(x, chain=True)
+        else:
+            sc = x
+        h = self.conv1(self.bn1.act(x, g1, b1), upsample=up)
+        return self.conv2(self.bn2.act(h, g2, b2), residual=sc, res_up=up)
 
     def _forward_sync(self, x, y, up, o1, o2):
         """Cross-replica BN: same arithmetic, launch order chosen so that each statistic all-reduce (latency-bound, on

@@ -1001,8 +1001,8 @@ class SNEmbeddingFn(Function):
             onehot = torch.zeros(n, sn.rows, device=dout.device, dtype=torch.float32)
             onehot.scatter_(1, flat.view(n, 1), 1.0)                  # (one element per row: no two writes meet)
             L.call("icg_gemm_batched", onehot, d2, dw_, sn.rows, sn.cin, n, 1, 0, 0, 0, 0, 1, 1.0)
-        else:     # a table too large for the one-hot form: ATen's sort-based (deterministic) embedding backward
-            dw_ = torch.ops.aten.embedding_dense_backward(d2, flat, sn.rows, -1, False)
+        else:     # a table too large for the one-hot form: by sorted labels, each label's samples in order as well
+            dw_ = embedding_backward(flat, d2, sn.rows)
         return None, _sn_backward(None, dw_, sn, ctx.weight_like), None
 
 
@@ -1427,6 +1427,16 @@ def attention(q, k, v, *, scale=None, causal=False, k_lens=None, q_start=None, r
     _require_gpu(q)
     o, lse = AttentionFn.apply(q, k, v, k_lens, q_start, scale, bool(causal))
     return (o, lse) if return_lse else o
+
+
+def image_attention(theta, phi, g):
+    """AttnCoreFn (reference layers.py:233-243) without the stored probabilities: theta [B, d, H, W], phi [B, d, h, w], g [B, dv, h, w]
+    -> [B, dv, H, W]; one head, unscaled scores, channels-last memory on both sides."""
+    theta, phi, g = _cl(theta), _cl(phi), _cl(g)
+    rows = lambda t: t.permute(0, 2, 3, 1).reshape(t.shape[0], -1, 1, t.shape[1])
+    o = attention(rows(theta), rows(phi), rows(g), scale=1.0)
+    B, _, H, W = theta.shape
+    return o.view(B, H, W, g.shape[1]).permute(0, 3, 1, 2)
 
 
 # ----------------------------------------------------------------------------------------------

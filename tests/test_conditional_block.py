@@ -1,0 +1,125 @@
+"""The operators as a generator uses them together: class embedding by sorted tokens -> conditional group norm + ReLU -> convolutions ->
+attention without stored probabilities, in G and D, forward and backward, against the 64-bit oracle (oracle/biggan_oracle.py with its conditional
+norm replaced by a group norm).  CPU: kernels emulated (wiring); GPU: the kernels."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from oracle import biggan_oracle as O, kernel_ref, synth
+from tests.helpers import DENSE_RMS_FRAC, GRAD_RTOL
+
+CFG = dict(dim_z=120, shared_dim=16, shared_dim_feat=32, G_shared=True, G_shared_feat=True, hier=True, n_classes=10, SN_eps=1e-6, BN_eps=1e-5,
+           adam_eps=1e-6, G_ch=8, D_ch=8, G_attn="32", D_attn="32", resolution=64, class_cond=True, instance_cond=True, DA=False)
+GROUPS = 8
+
+
+def _group_norm(sd, prefix, x, y, training, bn_eps, sn_eps):
+    gain = 1.0 + O.sn_linear(sd, prefix + ".gain", y, training, sn_eps)
+    bias = O.sn_linear(sd, prefix + ".bias", y, training, sn_eps)
+    return F.group_norm(x, GROUPS, eps=bn_eps) * gain.view(y.shape[0], -1, 1, 1) + bias.view(y.shape[0], -1, 1, 1)
+
+
+def _run(device, module, monkeypatch):
+    flags = dict(norm_style="gn_%d" % GROUPS, attn_recompute=True, sorted_embedding=True, skip_init=True, embedded_optimizers=False)
+    G, D = module.Generator(**{**CFG, **flags}), module.Discriminator(**{**CFG, **flags})
+    assert not any("stored_mean" in n for n, _ in G.named_buffers() if "output_layer" not in n)
+    for net, seed in ((G, 11), (D, 22)):
+        net.load_state_dict(synth.synth_state(synth.spec_of(net.state_dict()), seed))
+        for n, p in net.named_parameters():
+            if n.endswith("gamma"):                                      # (zero at the start: the attention's branch would not count)
+                p.data.fill_(0.7)
+    states = [{k: v.double().clone() for k, v in net.state_dict().items()} for net in (G, D)]
+    G, D = G.to(device).train(), D.to(device).train()
+    g = torch.Generator().manual_seed(5)
+    z, feats = torch.randn(6, G.dim_z, generator=g), F.normalize(torch.randn(6, 2048, generator=g), dim=1)
+    label = torch.tensor([3, 0, 3, 9, 3, 0])
+    up = torch.randn(6, 1, generator=g)
+    img = G(z.to(device), label.to(device), feats.to(device))
+    out = D(img, label.to(device), feats.to(device))
+    out.backward(up.to(device))
+    monkeypatch.setattr(O, "ccbn", _group_norm)
+    for sd, net in zip(states, (G, D)):
+        for n, _ in net.named_parameters():
+            sd[n].requires_grad_()
+    want_img = O.generator_forward(states[0], CFG, z.double(), label, feats.double())
+    want = O.discriminator_forward(states[1], CFG, want_img, label, feats.double())
+    want.backward(up.double())
+    return (G, D), states, (img, out), (want_img, want)
+
+
+def _compare(nets, states, got, want):
+    for a, b in zip(got, want):
+        b = b.detach()
+        assert float((a.detach().double().cpu() - b).norm()) <= 1e-4 * float(b.norm())
+    for net, sd in zip(nets, states):
+        rms = {n: float(sd[n].grad.square().mean().sqrt()) for n, _ in net.named_parameters()}
+        top = max(rms.values())
+        for n, p in net.named_parameters():
+            diff = float((p.grad.double().cpu() - sd[n].grad).square().mean().sqrt())
+            # the rms criterion of this repository's gradient comparisons (tests/helpers.py: fp32 against another evaluation of the same
+            # ReLU / max-pool network)
+            assert diff <= DENSE_RMS_FRAC * GRAD_RTOL * max(rms[n], 2e-3 * top), (n, diff, rms[n], top)
+        untouched = [r for r in range(CFG["n_classes"]) if r not in (0, 3, 9)]
+        if hasattr(net, "shared"):
+            assert not net.shared.weight.grad[untouched].any()
+
+
+def test_networks_with_the_operators_emulated(monkeypatch):
+    import ic_gan_amd.BigGAN as M
+    kernel_ref.install(monkeypatch)
+    _compare(*_run("cpu", M, monkeypatch))
+
+
+@pytest.mark.gpu
+def test_networks_with_the_operators(monkeypatch):
+    import ic_gan_amd.BigGAN as M
+    _compare(*_run("cuda", M, monkeypatch))
+
+
+@pytest.mark.gpu
+def test_recomputed_attention_block_equals_the_stored_one():
+    """layers.Attention, both modes: fp32 evaluations of the same formula in different orders.  Both are within 1e-5 of 64 bits at these
+    sizes (sums of up to 256 products of unit scale: n 2^-24), the weight gradients sum 2048 rows: 1e-4 of the tensor's norm."""
+    import copy
+    import functools
+    from ic_gan_amd import layers
+    conv = functools.partial(layers.SNConv2d, kernel_size=3, padding=1, num_svs=1, num_itrs=1, eps=1e-6)
+    a = layers.Attention(64, conv).cuda()
+    with torch.no_grad():
+        a.gamma.fill_(0.4)
+    b = copy.deepcopy(a)
+    b.recompute = True
+    x, dy = (torch.randn(2, 64, 32, 32, device="cuda").contiguous(memory_format=torch.channels_last) for _ in range(2))
+    out = []
+    for m in (a, b):
+        xi = x.clone().requires_grad_()
+        y = m(xi * 1.5)
+        y.backward(dy)
+        out.append([y.detach(), xi.grad] + [p.grad for p in m.parameters()])
+    for u, v in zip(*out):
+        assert float((u - v).norm()) <= 1e-4 * float(v.norm())
+
+
+@pytest.mark.gpu
+def test_deep_generator_with_group_norm():
+    import ic_gan_amd.BigGANdeep as M
+    cfg = dict(G_ch=16, dim_z=32, shared_dim=16, n_classes=10, hier=True, G_shared=True, resolution=32, G_attn="0", G_depth=2, norm_style="gn_2",
+               sorted_embedding=True, attn_recompute=True, no_optim=True)
+    G = M.Generator(**cfg).cuda().train()
+    y = torch.tensor([1, 2, 1], device="cuda")
+    img = G(torch.randn(3, G.dim_z, device="cuda"), G.shared(y))
+    img.square().mean().backward()
+    assert img.shape == (3, 3, 32, 32) and all(p.grad is not None and torch.isfinite(p.grad).all() for p in G.parameters())
+
+
+def test_norm_style_is_checked():
+    from ic_gan_amd import layers
+    import ic_gan_amd.BigGAN as M
+    for bad in ("in", "gn_", "gn_0", "gn_x", "ln"):
+        with pytest.raises(NotImplementedError):
+            M.Generator(**{**CFG, "norm_style": bad, "skip_init": True, "no_optim": True})
+    with pytest.raises(ValueError, match="groups over"):
+        M.Generator(**{**CFG, "norm_style": "gn_5", "skip_init": True, "no_optim": True})
+    assert layers.norm_groups("bn") is None and layers.norm_groups("gn") == 16 and layers.norm_groups("gn_32") == 32
+    with pytest.raises(NotImplementedError):
+        layers.Embedding(4, 4, sparse=True)
