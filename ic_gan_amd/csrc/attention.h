@@ -39,7 +39,7 @@ struct AttnP {
   int B, Lq, Lk, H, G, d, dv;               // H query heads, G of them to a key head
   int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
   float scale;
-  int causal, q_vec, k_vec, v_vec;          // *_vec: every row starts at a multiple of 16 bytes and holds whole 16-byte chunks
+  int causal;                               // (every row of q, k, v, o, do starts at a multiple of 16 bytes and holds whole 16-byte chunks)
   // forward
   void* o;
   float* lse;
@@ -48,7 +48,6 @@ struct AttnP {
   // gradient
   const void* dout;
   int64_t do_sb, do_sl, do_sh;
-  int do_vec;
   const float *stat;                        // [3][B][H][Lq]: l_i log2 e (less the shift of p), D_i, |do_i|
   void *dq, *dk, *dv_out;
   int tiles;                                // 32- or 128-row tiles of one head
@@ -111,36 +110,41 @@ struct at_tile {
   static __device__ __forceinline__ int at(int row, int chunk) { return row * STRIDE + ((chunk ^ ((row >> 2) & 3)) << 4); }
 };
 
-// 16 bytes of a row: elements PER c .. of `len`, zeros past the end.  Where rows are not whole aligned chunks, element by element.
-template <typename T>
-__device__ __forceinline__ at_u4 at_load_chunk(const T* row, int c, int len, bool vec) {
-  constexpr int PER = 16 / (int)sizeof(T);
-  at_u4 r = {0u, 0u, 0u, 0u};
-  if (vec) {
-    if (c * PER < len) r = *reinterpret_cast<const at_u4*>(row + c * PER);
-  } else {
-    T e[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) e[j] = c * PER + j < len ? row[c * PER + j] : (T)0.f;
-    __builtin_memcpy(&r, e, 16);
+// The registers of a streamed tile on its way from memory to LDS.  Loads go through a buffer descriptor of the tile's rows: a thread's
+// offsets within a tile never change, so a tile costs no address arithmetic in the lanes, and rows past the end read as zeros by the
+// descriptor's bound.  (A row's stride is at least its length, see at_row_ok.)
+struct at_rows {
+  uint64_t base;
+  uint32_t stride, len;                     // bytes
+  __device__ __forceinline__ at_rows(const void* p, int64_t stride_, int len_, int size)
+      : stride((uint32_t)(stride_ * size)), len((uint32_t)(len_ * size)) {
+    const uint64_t a = (uint64_t)p;
+    // (the builtin returns a signed int: without the casts a low half from 2^31 on would extend its sign over the high half)
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)), lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+    base = ((uint64_t)hi << 32) | lo;
   }
-  return r;
-}
+};
 
-// the registers of a tile on its way from memory to LDS: `fetch` starts the loads, `put` stores what arrived
 template <typename T, int E, int ROWS, int THREADS>
 struct at_stage {
   typedef at_tile<T, E> tile;
   static constexpr int N = (ROWS * tile::CHUNKS + THREADS - 1) / THREADS;
   static constexpr bool EXACT = (ROWS * tile::CHUNKS) % THREADS == 0;
   at_u4 r[N];
-  __device__ __forceinline__ void fetch(const T* base, int64_t stride, int row0, int rows_end, int len, bool vec, int tid) {
+  uint32_t off[N];
+  __device__ __forceinline__ at_stage(const at_rows& m, int tid) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int i = tid + n * THREADS, row = i / tile::CHUNKS, c = i - row * tile::CHUNKS;
-      r[n] = at_u4{0u, 0u, 0u, 0u};
-      if ((EXACT || row < ROWS) && row0 + row < rows_end) r[n] = at_load_chunk<T>(base + (int64_t)(row0 + row) * stride, c, len, vec);
+      off[n] = (EXACT || row < ROWS) && (uint32_t)c * 16u < m.len ? (uint32_t)row * m.stride + (uint32_t)c * 16u : 0x80000000u;
     }
+  }
+  __device__ __forceinline__ void fetch(const at_rows& m, int row0, int rows_end) {
+    const int rows = min(rows_end - row0, ROWS);
+    const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)(m.base + (uint64_t)row0 * m.stride), 0,
+                                                                       (int)((uint32_t)(rows - 1) * m.stride + m.len), 0x00027000);
+#pragma unroll
+    for (int n = 0; n < N; ++n) r[n] = __builtin_amdgcn_raw_buffer_load_b128(d, off[n], 0, 0);
   }
   __device__ __forceinline__ void put(char* lds, int tid) const {
 #pragma unroll
@@ -196,11 +200,13 @@ struct at_reader {
 
 // the wave's own 32 rows as column-side operands, straight from memory (used once per workgroup)
 template <typename T, int E>
-__device__ __forceinline__ void at_own(typename at_type<T>::frag (&f)[E / at_type<T>::KSTEP], const T* row, bool valid, int len, bool vec, int h) {
+__device__ __forceinline__ void at_own(typename at_type<T>::frag (&f)[E / at_type<T>::KSTEP], const T* row, bool valid, int len, int h) {
+  constexpr int PER = 16 / (int)sizeof(T);
 #pragma unroll
   for (int t = 0; t < E / at_type<T>::KSTEP; ++t) {
     at_u4 r = {0u, 0u, 0u, 0u};
-    if (valid) r = at_load_chunk<T>(row, 2 * t + h, len, vec);
+    const int c = (2 * t + h) * PER;
+    if (valid && c < len) r = *reinterpret_cast<const at_u4*>(row + c);
     f[t] = __builtin_bit_cast(typename at_type<T>::frag, r);
   }
 }
@@ -215,19 +221,13 @@ __device__ __forceinline__ float at_both_halves_sum(float v) {
 }
 __device__ __forceinline__ int at_row_of(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
-// four consecutive elements of an output row, as far as there are any
+// four consecutive elements of an output row (len is a multiple of 4)
 template <typename T>
 __device__ __forceinline__ void at_store4(T* row, int c, int len, float a, float b, float e, float f) {
-  T x[4] = {(T)a, (T)b, (T)e, (T)f};
-  if (len % 4 == 0) {                       // (the outputs are contiguous: their rows then start at multiples of 4 elements)
-    if (c < len) {
-      if constexpr (sizeof(T) == 2) { uint2 w; __builtin_memcpy(&w, x, 8); *reinterpret_cast<uint2*>(row + c) = w; }
-      else { at_u4 w; __builtin_memcpy(&w, x, 16); *reinterpret_cast<at_u4*>(row + c) = w; }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) if (c + j < len) row[c + j] = x[j];
-  }
+  if (c >= len) return;
+  const T x[4] = {(T)a, (T)b, (T)e, (T)f};
+  if constexpr (sizeof(T) == 2) { uint2 w; __builtin_memcpy(&w, x, 8); *reinterpret_cast<uint2*>(row + c) = w; }
+  else { at_u4 w; __builtin_memcpy(&w, x, 16); *reinterpret_cast<at_u4*>(row + c) = w; }
 }
 
 __device__ __forceinline__ int at_keys(const AttnP& p, int b) { return p.k_lens ? min(max(p.k_lens[b], 0), p.Lk) : p.Lk; }

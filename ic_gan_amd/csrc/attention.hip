@@ -32,12 +32,14 @@ bool at_shape_ok(int B, int Lq, int Lk, int H, int Hk, int d, int dv, int dtype)
   if (B <= 0 || Lq <= 0 || Lk <= 0 || H <= 0 || Hk <= 0 || H % Hk != 0) return false;
   if (dtype < 0 || dtype > 2) return false;
   if (Lq > (1 << 24) || Lk > (1 << 24) || H > (1 << 16) || (int64_t)B * H * Lq >= 0x7fffffffL || (int64_t)B * Hk * icg_cdiv(Lk, 128) >= 0x7fffffffL) return false;
-  return d > 0 && dv > 0 && ((d <= 128 && dv <= 128) || (d <= 64 && dv <= 256));
+  const int per = dtype == 0 ? 4 : 8;
+  return d > 0 && dv > 0 && d % per == 0 && dv % per == 0 && ((d <= 128 && dv <= 128) || (d <= 64 && dv <= 256));
 }
 
-bool at_row_vec(const void* x, int64_t sb, int64_t sl, int64_t sh, int len, int size) {
+// whole 16-byte chunks at multiples of 16 bytes; positions at least a row apart, and 128 of them within the reach of a descriptor
+bool at_row_ok(const void* x, int64_t sb, int64_t sl, int64_t sh, int len, int size) {
   const int per = 16 / size;
-  return ((uintptr_t)x % 16) == 0 && sb % per == 0 && sl % per == 0 && sh % per == 0 && len % per == 0;
+  return ((uintptr_t)x % 16) == 0 && sb % per == 0 && sl % per == 0 && sh % per == 0 && sl >= len && sl * size < (1 << 24);
 }
 
 }  // namespace
@@ -70,7 +72,7 @@ extern "C" int icg_attention_fwd(const void* q, const void* k, const void* v, co
   p.B = B, p.Lq = Lq, p.Lk = Lk, p.H = H, p.G = H / Hk, p.d = d, p.dv = dv;
   p.q_sb = q_sb, p.q_sl = q_sl, p.q_sh = q_sh, p.k_sb = k_sb, p.k_sl = k_sl, p.k_sh = k_sh, p.v_sb = v_sb, p.v_sl = v_sl, p.v_sh = v_sh;
   p.scale = scale, p.causal = causal != 0;
-  p.q_vec = at_row_vec(q, q_sb, q_sl, q_sh, d, size), p.k_vec = at_row_vec(k, k_sb, k_sl, k_sh, d, size), p.v_vec = at_row_vec(v, v_sb, v_sl, v_sh, dv, size);
+  ICG_REQUIRE(at_row_ok(q, q_sb, q_sl, q_sh, d, size) && at_row_ok(k, k_sb, k_sl, k_sh, d, size) && at_row_ok(v, v_sb, v_sl, v_sh, dv, size));
   at_plan(p, dtype);
   ICG_REQUIRE(p.work < 0x7fffffffL);
   if (p.nsplit > 1) {
@@ -101,8 +103,8 @@ extern "C" int icg_attention_bwd(const void* q, const void* k, const void* v, co
   p.q_sb = q_sb, p.q_sl = q_sl, p.q_sh = q_sh, p.k_sb = k_sb, p.k_sl = k_sl, p.k_sh = k_sh, p.v_sb = v_sb, p.v_sl = v_sl, p.v_sh = v_sh;
   p.do_sb = do_sb, p.do_sl = do_sl, p.do_sh = do_sh;
   p.scale = scale, p.causal = causal != 0;
-  p.q_vec = at_row_vec(q, q_sb, q_sl, q_sh, d, size), p.k_vec = at_row_vec(k, k_sb, k_sl, k_sh, d, size), p.v_vec = at_row_vec(v, v_sb, v_sl, v_sh, dv, size);
-  p.do_vec = at_row_vec(dout, do_sb, do_sl, do_sh, dv, size);
+  ICG_REQUIRE(at_row_ok(q, q_sb, q_sl, q_sh, d, size) && at_row_ok(k, k_sb, k_sl, k_sh, d, size) && at_row_ok(v, v_sb, v_sl, v_sh, dv, size));
+  ICG_REQUIRE(at_row_ok(dout, do_sb, do_sl, do_sh, dv, size));
   hipStream_t st = (hipStream_t)stream;
   float* stat = (float*)workspace;
   return dtype == 0 ? at_bwd_f32(p, stat, st) : dtype == 1 ? at_bwd_f16(p, stat, st) : at_bwd_bf16(p, stat, st);

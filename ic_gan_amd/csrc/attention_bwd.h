@@ -18,7 +18,7 @@ __global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, flo
   constexpr int PER = 16 / (int)sizeof(T);
   float dot = 0.f, sq = 0.f;
   for (int c = l; c * PER < p.dv; c += 32) {
-    const at_u4 a = at_load_chunk<T>(o, c, p.dv, (p.dv * sizeof(T)) % 16 == 0), e = at_load_chunk<T>(g, c, p.dv, p.do_vec);
+    const at_u4 a = *reinterpret_cast<const at_u4*>(o + c * PER), e = *reinterpret_cast<const at_u4*>(g + c * PER);
     T x[PER], y[PER];
     __builtin_memcpy(x, &a, 16);
     __builtin_memcpy(y, &e, 16);
@@ -49,8 +49,9 @@ __device__ __forceinline__ float at_ds(float pr, float dp, float s, float delta_
 }
 
 // dq: a workgroup owns 128 queries of one head (a wave 32, as columns) and streams the keys
+template <typename T, int DP, int DVP> constexpr int at_dq_waves() { return (DP + DVP) * (int)sizeof(T) / 8 + DP / 2 <= 160 ? 2 : 1; }
 template <typename T, int DP, int DVP>
-__global__ __launch_bounds__(256) void icg_attention_dq_kernel(AttnP p) {
+__global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attention_dq_kernel(AttnP p) {
   typedef at_type<T> X;
   typedef typename X::frag frag;
   constexpr int KT = sizeof(T) == 4 ? 32 : 64, KBYTES = KT * at_tile<T, DP>::STRIDE, SLOT = KBYTES + KT * at_tile<T, DVP>::STRIDE;
@@ -69,14 +70,14 @@ __global__ __launch_bounds__(256) void icg_attention_dq_kernel(AttnP p) {
   const int kend = p.causal ? min(keys, start + min(p.Lq - 1, 128 * tile + 127) + 1) : keys;
 
   frag qf[DP / X::KSTEP], gf[DVP / X::KSTEP];
-  at_own<T, DP>(qf, reinterpret_cast<const T*>(p.q) + b * p.q_sb + qi * p.q_sl + hq * p.q_sh, valid, p.d, p.q_vec, h);
-  at_own<T, DVP>(gf, reinterpret_cast<const T*>(p.dout) + b * p.do_sb + qi * p.do_sl + hq * p.do_sh, valid, p.dv, p.do_vec, h);
+  at_own<T, DP>(qf, reinterpret_cast<const T*>(p.q) + b * p.q_sb + qi * p.q_sl + hq * p.q_sh, valid, p.d, h);
+  at_own<T, DVP>(gf, reinterpret_cast<const T*>(p.dout) + b * p.do_sb + qi * p.do_sl + hq * p.do_sh, valid, p.dv, h);
   const int64_t rows = (int64_t)p.B * p.H * p.Lq, row = ((int64_t)b * p.H + hq) * p.Lq + qi;
   const float lse2 = valid ? p.stat[row] : INFINITY;
   const float s1 = X::SCALED && valid ? at_to_one(p.stat[2 * rows + row]) : 1.f;
   const float delta = valid ? p.stat[rows + row] * s1 : 0.f;
-  const T* kb = reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
-  const T* vb = reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  const at_rows kb(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_sl, p.d, sizeof(T));
+  const at_rows vb(reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_sl, p.dv, sizeof(T));
   const at_reader<T, DP> kr(lane);
   const at_reader<T, DVP> vr(lane);
   const float scl = p.scale * AT_LOG2E;
@@ -86,11 +87,11 @@ __global__ __launch_bounds__(256) void icg_attention_dq_kernel(AttnP p) {
   for (int c = 0; c < DP / 32; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[c][i] = 0.f;
-  at_stage<T, DP, KT, 256> ks;
-  at_stage<T, DVP, KT, 256> vs;
+  at_stage<T, DP, KT, 256> ks(kb, tid);
+  at_stage<T, DVP, KT, 256> vs(vb, tid);
   auto fetch = [&](int j) {
-    ks.fetch(kb, p.k_sl, j, kend, p.d, p.k_vec, tid);
-    vs.fetch(vb, p.v_sl, j, kend, p.dv, p.v_vec, tid);
+    ks.fetch(kb, j, kend);
+    vs.fetch(vb, j, kend);
   };
   auto put = [&](int cur) {
     ks.put(lds + cur * SLOT, tid);
@@ -148,8 +149,9 @@ __global__ __launch_bounds__(256) void icg_attention_dq_kernel(AttnP p) {
 
 // dk, dv: a workgroup owns 128 keys of one key head (a wave 32, as columns) and streams the queries of every head of the group, so the
 // gradient of a shared head is summed in registers
+template <typename T, int DP, int DVP> constexpr int at_dkv_waves() { return (DP + DVP) * ((int)sizeof(T) + 4) / 8 <= 192 ? 2 : 1; }
 template <typename T, int DP, int DVP>
-__global__ __launch_bounds__(256) void icg_attention_dkv_kernel(AttnP p) {
+__global__ __launch_bounds__(256, (at_dkv_waves<T, DP, DVP>())) void icg_attention_dkv_kernel(AttnP p) {
   typedef at_type<T> X;
   typedef typename X::frag frag;
   constexpr int QT = 32, QBYTES = QT * at_tile<T, DP>::STRIDE, GBYTES = QT * at_tile<T, DVP>::STRIDE, SLOT = QBYTES + GBYTES + 2 * QT * 4;
@@ -166,8 +168,8 @@ __global__ __launch_bounds__(256) void icg_attention_dkv_kernel(AttnP p) {
   const int64_t rows = (int64_t)p.B * p.H * p.Lq, row_b = ((int64_t)b * p.H + hk * p.G) * p.Lq;
 
   frag kf[DP / X::KSTEP], vf[DVP / X::KSTEP];
-  at_own<T, DP>(kf, reinterpret_cast<const T*>(p.k) + b * p.k_sb + j * p.k_sl + hk * p.k_sh, valid, p.d, p.k_vec, h);
-  at_own<T, DVP>(vf, reinterpret_cast<const T*>(p.v) + b * p.v_sb + j * p.v_sl + hk * p.v_sh, valid, p.dv, p.v_vec, h);
+  at_own<T, DP>(kf, reinterpret_cast<const T*>(p.k) + b * p.k_sb + j * p.k_sl + hk * p.k_sh, valid, p.d, h);
+  at_own<T, DVP>(vf, reinterpret_cast<const T*>(p.v) + b * p.v_sb + j * p.v_sl + hk * p.v_sh, valid, p.dv, h);
   const at_reader<T, DP> qr(lane);
   const at_reader<T, DVP> gr(lane);
   const float scl = p.scale * AT_LOG2E;
@@ -197,20 +199,25 @@ __global__ __launch_bounds__(256) void icg_attention_dkv_kernel(AttnP p) {
   // query i sees key j from i = j - start on
   const int i0 = p.causal ? max(0, 128 * tile - start) / QT : 0;
   const int per = max(0, (p.Lq + QT - 1) / QT - i0), n = 128 * tile < keys ? p.G * per : 0;
-  at_stage<T, DP, QT, 256> qs;
-  at_stage<T, DVP, QT, 256> gs;
+  at_rows qb(reinterpret_cast<const T*>(p.q) + b * p.q_sb + (int64_t)hk * p.G * p.q_sh, p.q_sl, p.d, sizeof(T));
+  at_rows gb(reinterpret_cast<const T*>(p.dout) + b * p.do_sb + (int64_t)hk * p.G * p.do_sh, p.do_sl, p.dv, sizeof(T));
+  at_stage<T, DP, QT, 256> qs(qb, tid);
+  at_stage<T, DVP, QT, 256> gs(gb, tid);
   float st = 0.f;                                        // threads 0 .. QT - 1: l_i, QT .. 2 QT - 1: D_i
   int fg = 0, ft = 0;                                    // head and tile of the next fetch
   auto fetch = [&]() {
-    const int r0 = (i0 + ft) * QT, hq = hk * p.G + fg;
-    qs.fetch(reinterpret_cast<const T*>(p.q) + b * p.q_sb + hq * p.q_sh, p.q_sl, r0, p.Lq, p.d, p.q_vec, tid);
-    gs.fetch(reinterpret_cast<const T*>(p.dout) + b * p.do_sb + hq * p.do_sh, p.do_sl, r0, p.Lq, p.dv, p.do_vec, tid);
+    const int r0 = (i0 + ft) * QT;
+    qs.fetch(qb, r0, p.Lq);
+    gs.fetch(gb, r0, p.Lq);
     if (tid < 2 * QT) {
       const int i = r0 + (tid & (QT - 1));
       const int64_t at = row_b + (int64_t)fg * p.Lq + i;
       st = tid < QT ? (i < p.Lq ? p.stat[at] : INFINITY) : (i < p.Lq ? p.stat[rows + at] * s1 : 0.f);
     }
-    if (++ft == per) ft = 0, ++fg;
+    if (++ft == per) {
+      ft = 0, ++fg;
+      qb.base += p.q_sh * sizeof(T), gb.base += p.do_sh * sizeof(T);
+    }
   };
   auto put = [&](int cur) {
     char* at = lds + cur * SLOT;

@@ -13,10 +13,12 @@ struct at_fwd_shape {
   static constexpr int KT = TOKENS ? 32 * WAVES : (sizeof(T) == 4 ? 32 : 64);
   static constexpr int SUB = TOKENS ? 1 : KT / 32;      // 32-key tiles of one wave
   static constexpr int BUFFERS = TOKENS ? 1 : 2;
+  // two waves per SIMD (256 registers) where own operands and sums leave room: one wave's exponentials run under the other's products
+  template <int DP, int DVP> static constexpr int waves() { return DP * (int)sizeof(T) / 8 + DVP / 2 <= (TOKENS ? 96 : 128) ? 2 : 1; }
 };
 
 template <typename T, int DP, int DVP, bool TOKENS>
-__global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS)) void icg_attention_fwd_kernel(AttnP p) {
+__global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS), (at_fwd_shape<T, TOKENS>::template waves<DP, DVP>())) void icg_attention_fwd_kernel(AttnP p) {
   typedef at_fwd_shape<T, TOKENS> S;
   typedef at_type<T> X;
   typedef typename X::frag frag;
@@ -64,9 +66,9 @@ __global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS)) void icg_attent
   }
 
   frag qf[DP / X::KSTEP];
-  at_own<T, DP>(qf, reinterpret_cast<const T*>(p.q) + b * p.q_sb + qi * p.q_sl + hq * p.q_sh, valid, p.d, p.q_vec, h);
-  const T* kb = reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
-  const T* vb = reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  at_own<T, DP>(qf, reinterpret_cast<const T*>(p.q) + b * p.q_sb + qi * p.q_sl + hq * p.q_sh, valid, p.d, h);
+  const at_rows kb(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_sl, p.d, sizeof(T));
+  const at_rows vb(reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_sl, p.dv, sizeof(T));
   const at_reader<T, DP> kr(lane);
   const at_reader<T, DVP> vr(lane);
 
@@ -78,19 +80,19 @@ __global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS)) void icg_attent
   float mx = AT_LOWEST, sum = 0.f;                       // running maximum (of s log2 e) and this half's part of the sum
   const float scl = p.scale * AT_LOG2E;
 
-  at_stage<T, DP, S::KT, S::THREADS> ks;
-  at_stage<T, DVP, S::KT, S::THREADS> vs;
+  at_stage<T, DP, S::KT, S::THREADS> ks(kb, tid);
+  at_stage<T, DVP, S::KT, S::THREADS> vs(vb, tid);
   if (k0 < kend) {
-    ks.fetch(kb, p.k_sl, k0, kend, p.d, p.k_vec, tid);
-    vs.fetch(vb, p.v_sl, k0, kend, p.dv, p.v_vec, tid);
+    ks.fetch(kb, k0, kend);
+    vs.fetch(vb, k0, kend);
   }
   int cur = 0;
   if (S::BUFFERS == 2 && k0 < kend) {
     ks.put(lds, tid);
     vs.put(lds + KBYTES, tid);
     if (k0 + S::KT < kend) {
-      ks.fetch(kb, p.k_sl, k0 + S::KT, kend, p.d, p.k_vec, tid);
-      vs.fetch(vb, p.v_sl, k0 + S::KT, kend, p.dv, p.v_vec, tid);
+      ks.fetch(kb, k0 + S::KT, kend);
+      vs.fetch(vb, k0 + S::KT, kend);
     }
     __syncthreads();
   }
@@ -100,8 +102,8 @@ __global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS)) void icg_attent
       ks.put(lds, tid);
       vs.put(lds + KBYTES, tid);
       if (j0 + S::KT < kend) {
-        ks.fetch(kb, p.k_sl, j0 + S::KT, kend, p.d, p.k_vec, tid);
-        vs.fetch(vb, p.v_sl, j0 + S::KT, kend, p.dv, p.v_vec, tid);
+        ks.fetch(kb, j0 + S::KT, kend);
+        vs.fetch(vb, j0 + S::KT, kend);
       }
       __syncthreads();
     }
@@ -161,8 +163,8 @@ __global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS)) void icg_attent
         ks.put(lds + cur * SLOT, tid);
         vs.put(lds + cur * SLOT + KBYTES, tid);
         if (j0 + 2 * S::KT < kend) {
-          ks.fetch(kb, p.k_sl, j0 + 2 * S::KT, kend, p.d, p.k_vec, tid);
-          vs.fetch(vb, p.v_sl, j0 + 2 * S::KT, kend, p.dv, p.v_vec, tid);
+          ks.fetch(kb, j0 + 2 * S::KT, kend);
+          vs.fetch(vb, j0 + 2 * S::KT, kend);
         }
         __syncthreads();
       }

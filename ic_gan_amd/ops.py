@@ -1328,9 +1328,17 @@ def _on_device(t: torch.Tensor):
     return torch.cuda.device(t.device) if t.is_cuda and t.get_device() != torch.cuda.current_device() else contextlib.nullcontext()
 
 
-def _rows_readable(t):
-    """the tensor itself if the kernels can address its rows (last dimension contiguous), else a contiguous copy"""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+def _rows_readable(t, width):
+    """the tensor itself if the attention kernels can address its rows (whole 16-byte chunks at multiples of 16 bytes, positions at least a row
+    and less than 16 MB apart), else a copy with rows of `width` elements, zeros behind"""
+    size, e = t.element_size(), t.shape[-1]
+    if e == width and (t.stride(-1) == 1 or e == 1) and t.data_ptr() % 16 == 0:
+        sb, sl, sh = t.stride(0), t.stride(1), t.stride(2)
+        if e <= sl < (1 << 24) // size and not (sb * size) % 16 and not (sl * size) % 16 and not (sh * size) % 16:
+            return t
+    if e == width:
+        return t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
+    return torch.nn.functional.pad(t, (0, width - e)).contiguous()
 
 
 def _strides3(t):
@@ -1356,7 +1364,10 @@ class AttentionFn(Function):
         B, Lq, H, d = q.shape
         Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
         dt = _DTYPE_CODES[q.dtype]
-        q, k, v = _rows_readable(q), _rows_readable(k), _rows_readable(v)
+        ctx.widths = (d, dv)
+        per = 16 // q.element_size()
+        d, dv = -(-d // per) * per, -(-dv // per) * per
+        q, k, v = _rows_readable(q, d), _rows_readable(k, d), _rows_readable(v, dv)
         o = torch.empty(B, Lq, H, dv, device=q.device, dtype=q.dtype)
         lse = torch.empty(B, H, Lq, device=q.device, dtype=torch.float32)
         if o.numel() == 0 or Lk == 0:
@@ -1370,7 +1381,7 @@ class AttentionFn(Function):
         ctx.scale, ctx.causal = scale, causal
         ctx.save_for_backward(q, k, v, o, lse, k_lens, q_start)
         ctx.mark_non_differentiable(lse)
-        return o, lse
+        return (o if dv == ctx.widths[1] else o[..., :ctx.widths[1]].contiguous()), lse
 
     @staticmethod
     @once_differentiable
@@ -1382,12 +1393,14 @@ class AttentionFn(Function):
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         dk, dv_ = torch.empty(k.shape, device=q.device, dtype=q.dtype), torch.empty(v.shape, device=q.device, dtype=q.dtype)
         if o.numel() == 0 or Lk == 0:
-            return dq.zero_(), dk.zero_(), dv_.zero_(), None, None, None, None
-        do = _rows_readable(do)
+            return dq.zero_()[..., :ctx.widths[0]], dk.zero_()[..., :ctx.widths[0]], dv_.zero_()[..., :ctx.widths[1]], None, None, None, None
+        do = _rows_readable(do, dv)
         with _on_device(q):
             nb = L.query("icg_attention_bwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, dt)
             L.call("icg_attention_bwd", q, k, v, o, do, lse, k_lens, q_start, dq, dk, dv_, B, Lq, Lk, H, Hk, d, dv, *_strides3(q), *_strides3(k),
                    *_strides3(v), *_strides3(do), ctx.scale, int(ctx.causal), dt, _bytes(nb, q.device), nb)
+        if ctx.widths != (d, dv):
+            dq, dk, dv_ = dq[..., :ctx.widths[0]], dk[..., :ctx.widths[0]], dv_[..., :ctx.widths[1]]
         return dq, dk, dv_, None, None, None, None
 
 
@@ -1422,7 +1435,7 @@ def attention(q, k, v, *, scale=None, causal=False, k_lens=None, q_start=None, r
     if not (0.0 < scale < float("inf")):
         raise ValueError("attention: scale must be positive and finite, not %r" % scale)
     k_lens, q_start = _check_index_vector("k_lens", k_lens, B, q), _check_index_vector("q_start", q_start, B, q)
-    if B * Lq * Lk and not L.query("icg_attention_applies", B, Lq, Lk, H, Hk, d, dv, _DTYPE_CODES[q.dtype]):
+    if B * Lq * Lk and not L.query("icg_attention_applies", B, Lq, Lk, H, Hk, -(-d // 8) * 8, -(-dv // 8) * 8, _DTYPE_CODES[q.dtype]):
         raise ValueError("attention: not served: B %d, Lq %d, Lk %d, H %d, d %d, dv %d (d, dv <= 128, or d <= 64 and dv <= 256)" % (B, Lq, Lk, H, d, dv))
     _require_gpu(q)
     o, lse = AttentionFn.apply(q, k, v, k_lens, q_start, scale, bool(causal))

@@ -788,11 +788,11 @@ int icg_sg2_torgb_bwd(const float* dimg, const void* y, const void* x, const flo
  *   s_ij = scale q_i . k_j   (seen: j < k_lens[b]; with `causal` also j <= q_start[b] + i),   l_i = log sum_j exp s_ij
  *   o_i = sum_j exp(s_ij - l_i) v_j           (a row that sees no key: o_i = 0, l_i = -inf)
  * and its gradient, which computes the probabilities again from q, k and l.  q [B][Lq][H][d], k [B][Lk][Hk][d], v [B][Lk][Hk][dv] with the
- * given element strides of batch, position and head (last dimension contiguous; any overlap is fine, they are only read); query head h
- * reads key head h / (H / Hk).  o, dq [B][Lq][H][..], dk, dv_out [B][Lk][Hk][..] contiguous, 16-byte aligned; lse [B][H][Lq] fp32.
+ * given element strides of batch, position and head (last dimension contiguous; rows are whole 16-byte chunks at multiples of 16 bytes,
+ * positions at least a row and less than 16 MB apart; heads and batches may overlap); query head h reads key head h / (H / Hk).  o, dq [B][Lq][H][..], dk, dv_out [B][Lk][Hk][..] contiguous, 16-byte aligned; lse [B][H][Lq] fp32.
  * dtype 0 / 1 / 2: fp32 / fp16 / bf16 (matrix products in that type, everything else in fp32).  k_lens, q_start: int32 [B] on the device or
  * NULL (Lk; Lk - Lq); keys from k_lens[b] on are not read, and their dk, dv are zero.  scale > 0.  `_applies`: d, dv <= 128, or d <= 64 and
- * dv <= 256.  A non-finite value that the causal mask hides from a query can still reach it (0 * inf); one from k_lens[b] on cannot. */
+ * dv <= 256, rows of whole 16-byte chunks.  A non-finite value that the causal mask hides from a query can still reach it (0 * inf); one from k_lens[b] on cannot. */
 int icg_attention_applies(int B, int Lq, int Lk, int H, int Hk, int d, int dv, int dtype);
 size_t icg_attention_fwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hk, int d, int dv, int dtype);
 int icg_attention_fwd(const void* q, const void* k, const void* v, const int* k_lens, const int* q_start, void* o, float* lse, int B, int Lq,
