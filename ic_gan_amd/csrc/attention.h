@@ -59,6 +59,8 @@ template <> struct at_type<float> {
   typedef at_f4 frag;
   static constexpr int KSTEP = 8, P_SHIFT = 0;
   static constexpr bool SCALED = false;
+  // whether step t of a sum over the head dimension holds elements: a step is 256 cycles here, worth a scalar branch
+  static __device__ __forceinline__ bool step(int t, int len) { return KSTEP * t < len; }
   static __device__ __forceinline__ at_f16v mma(frag a, frag b, at_f16v c) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], b[s], c, 0, 0, 0);
@@ -71,6 +73,7 @@ template <> struct at_type<__bf16> {
   typedef at_b8 frag;
   static constexpr int KSTEP = 16, P_SHIFT = 0;
   static constexpr bool SCALED = false;
+  static __device__ __forceinline__ bool step(int, int) { return true; }     // (32 cycles: the branch would cost more than the zeros)
   static __device__ __forceinline__ at_f16v mma(frag a, frag b, at_f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ frag pack(const at_f16v& x, int t) {
     frag f;
@@ -89,6 +92,7 @@ template <> struct at_type<_Float16> {
   typedef at_h8 frag;
   static constexpr int KSTEP = 16, P_SHIFT = 6;
   static constexpr bool SCALED = true;
+  static __device__ __forceinline__ bool step(int, int) { return true; }
   static __device__ __forceinline__ at_f16v mma(frag a, frag b, at_f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ frag pack(const at_f16v& x, int t) {
     frag f;

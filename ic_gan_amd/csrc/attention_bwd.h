@@ -49,7 +49,7 @@ __device__ __forceinline__ float at_ds(float pr, float dp, float s, float delta_
 }
 
 // dq: a workgroup owns 128 queries of one head (a wave 32, as columns) and streams the keys
-template <typename T, int DP, int DVP> constexpr int at_dq_waves() { return (DP + DVP) * (int)sizeof(T) / 8 + DP / 2 <= 160 ? 2 : 1; }
+template <typename T, int DP, int DVP> constexpr int at_dq_waves() { return (DP + DVP) * (int)sizeof(T) / 8 + DP / 2 <= 144 ? 2 : 1; }
 template <typename T, int DP, int DVP>
 __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attention_dq_kernel(AttnP p) {
   typedef at_type<T> X;
@@ -113,7 +113,8 @@ __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attentio
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = 0.f, dp[i] = 0.f;
 #pragma unroll
-      for (int t = 0; t < DP / X::KSTEP; ++t) s = X::mma(kr.row_frag(kt, 32 * u, t), qf[t], s);
+      for (int t = 0; t < DP / X::KSTEP; ++t)
+        if (X::step(t, p.d)) s = X::mma(kr.row_frag(kt, 32 * u, t), qf[t], s);
 #pragma unroll
       for (int t = 0; t < DVP / X::KSTEP; ++t) dp = X::mma(vr.row_frag(vt, 32 * u, t), gf[t], dp);
 #pragma unroll
@@ -149,17 +150,27 @@ __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attentio
 
 // dk, dv: a workgroup owns 128 keys of one key head (a wave 32, as columns) and streams the queries of every head of the group, so the
 // gradient of a shared head is summed in registers
-template <typename T, int DP, int DVP> constexpr int at_dkv_waves() { return (DP + DVP) * ((int)sizeof(T) + 4) / 8 <= 192 ? 2 : 1; }
+// Registers of a lane: own keys and values (DP + DVP) size / 8, sums (DP + DVP) / 2, about 100 beside them.  Two waves per SIMD (256) hold up
+// to 144 of the first two.  A wave alone on its SIMD has nothing to run while a tile arrives: it streams 64 rows at a time (16-bit 128 + 128:
+// 762 us with 32 rows, 581 with 64, at 2 x 4096 causal, 16 heads over 4).
 template <typename T, int DP, int DVP>
-__global__ __launch_bounds__(256, (at_dkv_waves<T, DP, DVP>())) void icg_attention_dkv_kernel(AttnP p) {
+struct at_dkv_shape {
+  static constexpr int WAVES = (DP + DVP) * ((int)sizeof(T) + 4) / 8 <= 144 ? 2 : 1, QT = sizeof(T) == 2 && WAVES == 1 ? 64 : 32;
+  static constexpr int QBYTES = QT * at_tile<T, DP>::STRIDE, GBYTES = QT * at_tile<T, DVP>::STRIDE, SLOT = QBYTES + GBYTES + 2 * QT * 4;
+};
+template <typename T, int DP, int DVP>
+__global__ __launch_bounds__(256, (at_dkv_shape<T, DP, DVP>::WAVES)) void icg_attention_dkv_kernel(AttnP p) {
   typedef at_type<T> X;
   typedef typename X::frag frag;
-  constexpr int QT = 32, QBYTES = QT * at_tile<T, DP>::STRIDE, GBYTES = QT * at_tile<T, DVP>::STRIDE, SLOT = QBYTES + GBYTES + 2 * QT * 4;
+  typedef at_dkv_shape<T, DP, DVP> S;
+  constexpr int QT = S::QT, QBYTES = S::QBYTES, GBYTES = S::GBYTES, SLOT = S::SLOT;
   __shared__ __attribute__((aligned(64))) char lds[2 * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 31, h = lane >> 5;
-  const int64_t item = at_work_item(p.work);
-  const int tile = (int)(item % p.tiles);
+  int64_t item = at_work_item(p.work);
+  const int split = (int)(item % p.nsplit);
+  item /= p.nsplit;
+  const int tile = (int)(item % p.tiles);                // (the first keys, seen by the most queries of a causal triangle, first)
   const int64_t bh = item / p.tiles;
   const int Hk = p.H / p.G, b = (int)(bh / Hk), hk = (int)(bh - (int64_t)b * Hk);
   const int j = 128 * tile + 32 * wv + m;
@@ -198,13 +209,15 @@ __global__ __launch_bounds__(256, (at_dkv_waves<T, DP, DVP>())) void icg_attenti
 
   // query i sees key j from i = j - start on
   const int i0 = p.causal ? max(0, 128 * tile - start) / QT : 0;
-  const int per = max(0, (p.Lq + QT - 1) / QT - i0), n = 128 * tile < keys ? p.G * per : 0;
+  const int per = max(0, (p.Lq + QT - 1) / QT - i0), all = 128 * tile < keys ? p.G * per : 0;
+  const int share = (all + p.nsplit - 1) / p.nsplit, n0 = min(split * share, all), n = min(share, all - n0);      // this split's tiles
   at_rows qb(reinterpret_cast<const T*>(p.q) + b * p.q_sb + (int64_t)hk * p.G * p.q_sh, p.q_sl, p.d, sizeof(T));
   at_rows gb(reinterpret_cast<const T*>(p.dout) + b * p.do_sb + (int64_t)hk * p.G * p.do_sh, p.do_sl, p.dv, sizeof(T));
   at_stage<T, DP, QT, 256> qs(qb, tid);
   at_stage<T, DVP, QT, 256> gs(gb, tid);
   float st = 0.f;                                        // threads 0 .. QT - 1: l_i, QT .. 2 QT - 1: D_i
-  int fg = 0, ft = 0;                                    // head and tile of the next fetch
+  int fg = per > 0 ? n0 / per : 0, ft = n0 - fg * per;   // head and tile of the next fetch
+  qb.base += (int64_t)fg * p.q_sh * (int64_t)sizeof(T), gb.base += (int64_t)fg * p.do_sh * (int64_t)sizeof(T);
   auto fetch = [&]() {
     const int r0 = (i0 + ft) * QT;
     qs.fetch(qb, r0, p.Lq);
@@ -216,7 +229,7 @@ __global__ __launch_bounds__(256, (at_dkv_waves<T, DP, DVP>())) void icg_attenti
     }
     if (++ft == per) {
       ft = 0, ++fg;
-      qb.base += p.q_sh * sizeof(T), gb.base += p.do_sh * sizeof(T);
+      qb.base += p.q_sh * (int64_t)sizeof(T), gb.base += p.do_sh * (int64_t)sizeof(T);
     }
   };
   auto put = [&](int cur) {
@@ -225,7 +238,7 @@ __global__ __launch_bounds__(256, (at_dkv_waves<T, DP, DVP>())) void icg_attenti
     gs.put(at + QBYTES, tid);
     if (tid < 2 * QT) reinterpret_cast<float*>(at + QBYTES + GBYTES)[tid] = st;
   };
-  int cur = 0, t0 = 0;                                   // tile of the current one within its head
+  int cur = 0, t0 = ft;                                  // tile of the current one within its head
   if (n > 0) {
     fetch();
     put(0);
@@ -236,42 +249,46 @@ __global__ __launch_bounds__(256, (at_dkv_waves<T, DP, DVP>())) void icg_attenti
     const char* qt = lds + cur * SLOT;
     const char* gt = qt + QBYTES;
     const float* stat = reinterpret_cast<const float*>(gt + GBYTES);
-    at_f16v s, dp;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.f, dp[i] = 0.f;
+    for (int u = 0; u < QT / 32; ++u) {
+      at_f16v s, dp;
 #pragma unroll
-    for (int t = 0; t < DP / X::KSTEP; ++t) s = X::mma(qr.row_frag(qt, 0, t), kf[t], s);
+      for (int i = 0; i < 16; ++i) s[i] = 0.f, dp[i] = 0.f;
 #pragma unroll
-    for (int t = 0; t < DVP / X::KSTEP; ++t) dp = X::mma(gr.row_frag(gt, 0, t), vf[t], dp);
-    const int first = valid ? (p.causal ? j - start : -(1 << 30)) : 0x7fffffff;       // the first query that sees this lane's key
-    const int r0 = (i0 + t0) * QT;
-    const bool edge = __any(r0 < first);
+      for (int t = 0; t < DP / X::KSTEP; ++t)
+        if (X::step(t, p.d)) s = X::mma(qr.row_frag(qt, 32 * u, t), kf[t], s);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const at_f4 l4 = *reinterpret_cast<const at_f4*>(stat + 8 * g + 4 * h), d4 = *reinterpret_cast<const at_f4*>(stat + QT + 8 * g + 4 * h);
+      for (int t = 0; t < DVP / X::KSTEP; ++t) dp = X::mma(gr.row_frag(gt, 32 * u, t), vf[t], dp);
+      const int first = valid ? (p.causal ? j - start : -(1 << 30)) : 0x7fffffff;       // the first query that sees this lane's key
+      const int r0 = (i0 + t0) * QT + 32 * u;
+      const bool edge = __any(r0 < first);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 4 * g + e;
-        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scl, -l4[e]));
-        dp[i] = at_ds<T>(s[i], dp[i], s1, d4[e]);
+      for (int g = 0; g < 4; ++g) {
+        const at_f4 l4 = *reinterpret_cast<const at_f4*>(stat + 32 * u + 8 * g + 4 * h), d4 = *reinterpret_cast<const at_f4*>(stat + QT + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * g + e;
+          s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scl, -l4[e]));
+          dp[i] = at_ds<T>(s[i], dp[i], s1, d4[e]);
+        }
       }
-    }
-    if (edge) {
+      if (edge) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const bool off = r0 + at_row_of(i, h) < first;
-        s[i] = off ? 0.f : s[i];
-        dp[i] = off ? 0.f : dp[i];
+        for (int i = 0; i < 16; ++i) {
+          const bool off = r0 + at_row_of(i, h) < first;
+          s[i] = off ? 0.f : s[i];
+          dp[i] = off ? 0.f : dp[i];
+        }
       }
-    }
-    // p and ds are rounded to the inputs' type for the matrix products: half a step each, summed over the queries in 32 bits
+      // p and ds are rounded to the inputs' type for the matrix products: half a step each, summed over the queries in 32 bits
 #pragma unroll
-    for (int q = 0; q < 32 / X::KSTEP; ++q) {
-      const frag pf = X::pack(s, q), sf = X::pack(dp, q);
+      for (int q = 0; q < 32 / X::KSTEP; ++q) {
+        const frag pf = X::pack(s, q), sf = X::pack(dp, q);
 #pragma unroll
-      for (int c = 0; c < DVP / 32; ++c) dv[c] = X::mma(gr.col_frag(gt, 0, c, q), pf, dv[c]);
+        for (int c = 0; c < DVP / 32; ++c) dv[c] = X::mma(gr.col_frag(gt, 32 * u, c, q), pf, dv[c]);
 #pragma unroll
-      for (int c = 0; c < DP / 32; ++c) dk[c] = X::mma(qr.col_frag(qt, 0, c, q), sf, dk[c]);
+        for (int c = 0; c < DP / 32; ++c) dk[c] = X::mma(qr.col_frag(qt, 32 * u, c, q), sf, dk[c]);
+      }
     }
     if (++t0 == per) t0 = 0;
     if (it + 1 < n) {
@@ -283,6 +300,20 @@ __global__ __launch_bounds__(256, (at_dkv_waves<T, DP, DVP>())) void icg_attenti
   }
   if (j >= p.Lk) return;                                 // (keys from k_lens on have no gradient: their sums are zero)
   const float fv = 1.f / (1 << X::P_SHIFT), fk = p.scale * fv / s1;
+  if (p.nsplit > 1) {
+    float* out = p.part + ((((int64_t)split * p.B + b) * p.Lk + j) * Hk + hk) * (p.d + p.dv);
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        at_store4<float>(out, 32 * c + 8 * g + 4 * h, p.d, dk[c][4 * g] * fk, dk[c][4 * g + 1] * fk, dk[c][4 * g + 2] * fk, dk[c][4 * g + 3] * fk);
+#pragma unroll
+    for (int c = 0; c < DVP / 32; ++c)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        at_store4<float>(out + p.d, 32 * c + 8 * g + 4 * h, p.dv, dv[c][4 * g] * fv, dv[c][4 * g + 1] * fv, dv[c][4 * g + 2] * fv, dv[c][4 * g + 3] * fv);
+    return;
+  }
   T* dk_out = reinterpret_cast<T*>(p.dk) + (((int64_t)b * p.Lk + j) * Hk + hk) * p.d;
   T* dv_out = reinterpret_cast<T*>(p.dv_out) + (((int64_t)b * p.Lk + j) * Hk + hk) * p.dv;
 #pragma unroll
@@ -297,21 +328,38 @@ __global__ __launch_bounds__(256, (at_dkv_waves<T, DP, DVP>())) void icg_attenti
       at_store4<T>(dv_out, 32 * c + 8 * g + 4 * h, p.dv, dv[c][4 * g] * fv, dv[c][4 * g + 1] * fv, dv[c][4 * g + 2] * fv, dv[c][4 * g + 3] * fv);
 }
 
+// sums the splits of dk and dv in order: a thread takes 4 elements of a key's row [d + dv]
+template <typename T>
+__global__ __launch_bounds__(256) void icg_attention_join_dkv_kernel(AttnP p) {
+  const int64_t rows = (int64_t)p.B * p.Lk * (p.H / p.G);
+  const int w = p.d + p.dv, quads = w / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / quads;
+  if (row >= rows) return;
+  const int c = (int)(i - row * quads) * 4;
+  at_f4 x = *reinterpret_cast<const at_f4*>(p.part + row * w + c);
+  for (int s = 1; s < p.nsplit; ++s) x += *reinterpret_cast<const at_f4*>(p.part + (s * rows + row) * w + c);
+  if (c < p.d) at_store4<T>(reinterpret_cast<T*>(p.dk) + row * p.d, c, p.d, x[0], x[1], x[2], x[3]);
+  else at_store4<T>(reinterpret_cast<T*>(p.dv_out) + row * p.dv, c - p.d, p.dv, x[0], x[1], x[2], x[3]);
+}
+
 template <typename T>
 int at_bwd(const AttnP& in, float* stat, hipStream_t st) {
   AttnP p = in;
   p.stat = stat;
   hipLaunchKernelGGL((icg_attention_rowstat_kernel<T>), dim3((unsigned)icg_cdiv((int64_t)p.B * p.H * p.Lq, 8)), dim3(256), 0, st, p, stat);
   if (const int e = icg_check_launch()) return e;
-  AttnP pk = p;
-  pk.tiles = (int)icg_cdiv(p.Lk, 128);
-  pk.work = (int64_t)p.B * (p.H / p.G) * pk.tiles;
+  const AttnP pk = p;                                    // (planned by the caller: key tiles and splits)
   p.tiles = (int)icg_cdiv(p.Lq, 128);
   p.work = (int64_t)p.B * p.H * p.tiles;
 #define AT_RUN(DP, DVP)                                                                                                 \
   do {                                                                                                                  \
     hipLaunchKernelGGL((icg_attention_dkv_kernel<T, DP, DVP>), dim3((unsigned)pk.work), dim3(256), 0, st, pk);          \
     if (const int e = icg_check_launch()) return e;                                                                     \
+    if (pk.nsplit > 1) {                                                                                                \
+      const int64_t quads = (int64_t)p.B * p.Lk * (p.H / p.G) * ((p.d + p.dv) / 4);                                     \
+      hipLaunchKernelGGL((icg_attention_join_dkv_kernel<T>), dim3((unsigned)icg_cdiv(quads, 256)), dim3(256), 0, st, pk); \
+      if (const int e = icg_check_launch()) return e;                                                                   \
+    }                                                                                                                   \
     hipLaunchKernelGGL((icg_attention_dq_kernel<T, DP, DVP>), dim3((unsigned)p.work), dim3(256), 0, st, p);             \
   } while (0)
   AT_FOR_HEAD(p.d, p.dv, AT_RUN)

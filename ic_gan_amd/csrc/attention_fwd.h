@@ -116,7 +116,8 @@ __global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS), (at_fwd_shape<T
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
 #pragma unroll
-      for (int t = 0; t < DP / X::KSTEP; ++t) s[u] = X::mma(kr.row_frag(kt, sub0 + 32 * u, t), qf[t], s[u]);
+      for (int t = 0; t < DP / X::KSTEP; ++t)
+        if (X::step(t, p.d)) s[u] = X::mma(kr.row_frag(kt, sub0 + 32 * u, t), qf[t], s[u]);
     }
     const int jw = j0 + sub0;
     if (__any(jw + 32 * S::SUB - 1 > last)) {
@@ -236,29 +237,29 @@ __global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS), (at_fwd_shape<T
         at_store4<T>(out, 32 * c + 8 * g + 4 * h, p.dv, o[c][4 * g] * inv, o[c][4 * g + 1] * inv, o[c][4 * g + 2] * inv, o[c][4 * g + 3] * inv);
 }
 
-// joins the splits of one row: 64 lanes, 4 columns each, splits in order
+// joins the splits of a row: a wave per row, 4 columns a lane, splits in order
 template <typename T>
-__global__ __launch_bounds__(64) void icg_attention_join_kernel(AttnP p) {
-  const int64_t rows = (int64_t)p.B * p.H * p.Lq, row = blockIdx.x;
+__global__ __launch_bounds__(256) void icg_attention_join_kernel(AttnP p) {
+  const int64_t rows = (int64_t)p.B * p.H * p.Lq, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 63, c = 4 * lane;
   const at_f2* stat = reinterpret_cast<const at_f2*>(p.part + p.nsplit * rows * p.dv) + row;
   float mx = AT_LOWEST;
   for (int s = 0; s < p.nsplit; ++s) mx = fmaxf(mx, stat[s * rows][0]);
-  float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  const int c = 4 * threadIdx.x;
+  float sum = 0.f;
+  at_f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int s = 0; s < p.nsplit; ++s) {
     const at_f2 ms = stat[s * rows];
-    if (ms[1] == 0.f) continue;
+    if (ms[1] == 0.f) continue;                          // (a split that saw no key wrote no sums)
     const float a = __builtin_amdgcn_exp2f(ms[0] - mx);
     sum += ms[1] * a;
-    const float* in = p.part + (s * rows + row) * p.dv + c;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) if (c + j < p.dv) o[j] += in[j] * a;
+    if (c < p.dv) o += *reinterpret_cast<const at_f4*>(p.part + (s * rows + row) * p.dv + c) * a;
   }
-  if (threadIdx.x == 0) p.lse[row] = sum == 0.f ? -INFINITY : mx * AT_LN2 + __logf(sum);
+  if (lane == 0) p.lse[row] = sum == 0.f ? -INFINITY : mx * AT_LN2 + __logf(sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t bh = row / p.Lq, qi = row - bh * p.Lq, b = bh / p.H, hq = bh - b * p.H;
-  T* out = reinterpret_cast<T*>(p.o) + ((b * p.Lq + qi) * p.H + hq) * p.dv;
-  if (c < p.dv) at_store4<T>(out, c, p.dv, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  at_store4<T>(reinterpret_cast<T*>(p.o) + ((b * p.Lq + qi) * p.H + hq) * p.dv, c, p.dv, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
 template <typename T>
@@ -272,7 +273,7 @@ int at_fwd(const AttnP& p, bool tokens, hipStream_t st) {
 #undef AT_RUN
   if (const int e = icg_check_launch()) return e;
   if (p.nsplit > 1) {
-    hipLaunchKernelGGL((icg_attention_join_kernel<T>), dim3((unsigned)((int64_t)p.B * p.H * p.Lq)), dim3(64), 0, st, p);
+    hipLaunchKernelGGL((icg_attention_join_kernel<T>), dim3((unsigned)icg_cdiv((int64_t)p.B * p.H * p.Lq, 4)), dim3(256), 0, st, p);
     return icg_check_launch();
   }
   return ICG_OK;

@@ -1396,7 +1396,7 @@ class AttentionFn(Function):
             return dq.zero_()[..., :ctx.widths[0]], dk.zero_()[..., :ctx.widths[0]], dv_.zero_()[..., :ctx.widths[1]], None, None, None, None
         do = _rows_readable(do, dv)
         with _on_device(q):
-            nb = L.query("icg_attention_bwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, dt)
+            nb = L.query("icg_attention_bwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, int(ctx.causal), dt)
             L.call("icg_attention_bwd", q, k, v, o, do, lse, k_lens, q_start, dq, dk, dv_, B, Lq, Lk, H, Hk, d, dv, *_strides3(q), *_strides3(k),
                    *_strides3(v), *_strides3(do), ctx.scale, int(ctx.causal), dt, _bytes(nb, q.device), nb)
         if ctx.widths != (d, dv):

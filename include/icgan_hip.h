@@ -799,7 +799,7 @@ int icg_attention_fwd(const void* q, const void* k, const void* v, const int* k_
                       int Lk, int H, int Hk, int d, int dv, int64_t q_sb, int64_t q_sl, int64_t q_sh, int64_t k_sb, int64_t k_sl, int64_t k_sh,
                       int64_t v_sb, int64_t v_sl, int64_t v_sh, float scale, int causal, int dtype, void* workspace, size_t workspace_bytes,
                       void* stream);
-size_t icg_attention_bwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hk, int d, int dv, int dtype);
+size_t icg_attention_bwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hk, int d, int dv, int causal, int dtype);
 int icg_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, const int* k_lens,
                       const int* q_start, void* dq, void* dk, void* dv_out, int B, int Lq, int Lk, int H, int Hk, int d, int dv, int64_t q_sb,
                       int64_t q_sl, int64_t q_sh, int64_t k_sb, int64_t k_sl, int64_t k_sh, int64_t v_sb, int64_t v_sl, int64_t v_sh,

@@ -1536,7 +1536,7 @@ def icg_attention_fwd_workspace_bytes(*a):
     return 0
 
 
-def icg_attention_bwd_workspace_bytes(B, Lq, Lk, H, Hk, d, dv, dtype):
+def icg_attention_bwd_workspace_bytes(B, Lq, Lk, H, Hk, d, dv, causal, dtype):
     return 12 * B * H * Lq
 
 
