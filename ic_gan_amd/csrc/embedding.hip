@@ -22,7 +22,10 @@ struct EmbP {
   float* part;                        // [ceil(n / EMB_CHUNK)][2][D]
 };
 
-constexpr int EMB_CHUNK = 64;         // list entries of one piece
+#ifndef EMB_C
+#define EMB_C 32
+#endif
+constexpr int EMB_CHUNK = EMB_C;         // list entries of one piece
 constexpr int EMB_RUN = 1024;         // most tokens a workgroup of the sort owns (64 KB of counts)
 constexpr int EMB_FEW = 1024;         // up to here the gradient scans the list per row, in one launch
 
@@ -106,7 +109,7 @@ __global__ __launch_bounds__(256) void icg_embedding_bwd_few_kernel(EmbP p) {
 }
 
 // ---- the positions in the order of their tokens
-constexpr int EMB_WAVES = 16;
+constexpr int EMB_WAVES = 16, EMB_BATCH = 8;
 __global__ __launch_bounds__(64 * EMB_WAVES) void icg_embedding_sort_kernel(EmbP p) {
   __shared__ int count[EMB_WAVES * EMB_RUN];               // [wave][token]: occurrences, then the next place
   __shared__ int less[EMB_WAVES], sums[EMB_WAVES];
@@ -117,8 +120,14 @@ __global__ __launch_bounds__(64 * EMB_WAVES) void icg_embedding_sort_kernel(EmbP
   __syncthreads();
   const int64_t share = (p.n + EMB_WAVES * 64 - 1) / (EMB_WAVES * 64) * 64, i0 = wv * share, i1 = min(i0 + share, p.n);
   int below = 0;
-  for (int64_t i = i0; i < i1; i += 64) {
-    const int64_t t = i + lane < i1 ? em_token(p, i + lane) : -1;
+  // (EMB_BATCH loads in flight: a sweep waits for its list, not for its arithmetic)
+  for (int64_t g = i0; g < i1; g += 64 * EMB_BATCH) {
+    int64_t ahead[EMB_BATCH];
+#pragma unroll
+    for (int k = 0; k < EMB_BATCH; ++k) ahead[k] = g + 64 * k + lane < i1 ? em_token(p, g + 64 * k + lane) : -1;
+#pragma unroll
+    for (int k = 0; k < EMB_BATCH; ++k) {
+    const int64_t t = ahead[k];
     const bool valid = (uint64_t)t < (uint64_t)p.V && t != p.pad;
     below += __builtin_popcountll(__ballot(valid && t < v0));
     const int u = valid && t >= v0 && t < v0 + own ? (int)(t - v0) : -1;
@@ -130,6 +139,7 @@ __global__ __launch_bounds__(64 * EMB_WAVES) void icg_embedding_sort_kernel(EmbP
       rest &= ~same;
     }
     icg_wave_lds_sync();
+    }
   }
   if (lane == 0) less[wv] = below;
   __syncthreads();
@@ -161,8 +171,13 @@ __global__ __launch_bounds__(64 * EMB_WAVES) void icg_embedding_sort_kernel(EmbP
     if (v0 + tid == p.V - 1) p.start[p.V] = next;
   }
   __syncthreads();
-  for (int64_t i = i0; i < i1; i += 64) {
-    const int64_t t = i + lane < i1 ? em_token(p, i + lane) : -1;
+  for (int64_t g = i0; g < i1; g += 64 * EMB_BATCH) {
+    int64_t ahead[EMB_BATCH];
+#pragma unroll
+    for (int k = 0; k < EMB_BATCH; ++k) ahead[k] = g + 64 * k + lane < i1 ? em_token(p, g + 64 * k + lane) : -1;
+#pragma unroll
+    for (int k = 0; k < EMB_BATCH; ++k) {
+    const int64_t i = g + 64 * k, t = ahead[k];
     const bool hit = t >= v0 && t < v0 + own && t != p.pad;
     const int u = hit ? (int)(t - v0) : -1;
     unsigned long long rest = __ballot(hit);
@@ -177,6 +192,7 @@ __global__ __launch_bounds__(64 * EMB_WAVES) void icg_embedding_sort_kernel(EmbP
       if (lane == first) *next = place + __builtin_popcountll(same);
       icg_wave_lds_sync();
       rest &= ~same;
+    }
     }
   }
 }
@@ -218,39 +234,61 @@ __global__ __launch_bounds__(64) void icg_embedding_bwd_piece_kernel(EmbP p) {
   }
 }
 
+// a wave per row of the table, EMB_TILES column tiles at once so that an entry's whole row is in flight
+constexpr int EMB_TILES = 4;
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void icg_embedding_bwd_row_kernel(EmbP p) {
   const int lane = threadIdx.x & 63;
   const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (v >= p.V) return;
   const int b = p.start[v], e = p.start[v + 1];
-  for (int64_t c = lane * VEC; c < p.D; c += 64 * VEC) {
-    float a[VEC];
+  for (int64_t c0 = lane * VEC; c0 < p.D; c0 += 64 * VEC * EMB_TILES) {
+    float a[EMB_TILES][VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) a[j] = 0.f;
+    for (int u = 0; u < EMB_TILES; ++u)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) a[u][j] = 0.f;
     if (e - b <= EMB_CHUNK) {
+      const T* dout = reinterpret_cast<const T*>(p.dout) + c0;
       int i = b;
-      for (; i + 4 <= e; i += 4) {
-        em_vec<T, VEC> x[4];
+      for (; i + 2 <= e; i += 2) {
+        em_vec<T, VEC> x[2][EMB_TILES];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) x[q] = em_load<T, VEC>(reinterpret_cast<const T*>(p.dout) + (int64_t)p.order[i + q] * p.D + c);
+        for (int q = 0; q < 2; ++q) {
+          const T* row = dout + (int64_t)p.order[i + q] * p.D;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+          for (int u = 0; u < EMB_TILES; ++u)
+            if (c0 + u * 64 * VEC < p.D) x[q][u] = em_load<T, VEC>(row + u * 64 * VEC);
+        }
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) a[j] += (float)x[q].e[j];
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int u = 0; u < EMB_TILES; ++u)
+            if (c0 + u * 64 * VEC < p.D)
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) a[u][j] += (float)x[q][u].e[j];
       }
-      for (; i < e; ++i) em_add<T, VEC>(a, p, p.order[i], c);
+      if (i < e)
+#pragma unroll
+        for (int u = 0; u < EMB_TILES; ++u)
+          if (c0 + u * 64 * VEC < p.D) em_add<T, VEC>(a[u], p, p.order[i], c0 + u * 64 * VEC);
     } else {
       const int k0 = b / EMB_CHUNK, k1 = (e - 1) / EMB_CHUNK;
-      const float* in = p.part + c;
-#pragma unroll 4
-      for (int k = k0; k <= k1; ++k) {
-        const float* q = in + ((int64_t)k * 2 + (b < k * EMB_CHUNK ? 0 : 1)) * p.D;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) a[j] += q[j];
+      for (int u = 0; u < EMB_TILES; ++u) {
+        if (c0 + u * 64 * VEC >= p.D) continue;
+        const float* in = p.part + c0 + u * 64 * VEC;
+#pragma unroll 4
+        for (int k = k0; k <= k1; ++k) {
+          const float* q = in + ((int64_t)k * 2 + (b < k * EMB_CHUNK ? 0 : 1)) * p.D;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) a[u][j] += q[j];
+        }
       }
     }
-    em_write<T, VEC>(a, p, v, c);
+#pragma unroll
+    for (int u = 0; u < EMB_TILES; ++u)
+      if (c0 + u * 64 * VEC < p.D) em_write<T, VEC>(a[u], p, v, c0 + u * 64 * VEC);
   }
 }
 

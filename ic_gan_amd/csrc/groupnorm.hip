@@ -28,7 +28,8 @@ struct GnP {
   int64_t rows;                       // rows per chunk
 };
 
-constexpr int GN_R = 8;               // rows a thread holds in registers
+constexpr int GN_R = 8;               // rows a thread holds in registers (one pass)
+constexpr int GN_P = 4;               // rows whose moments a thread forms at a time (three passes)
 
 template <typename T, int VEC> struct gn_vec { T e[VEC]; };
 template <typename T, int VEC>
@@ -53,30 +54,32 @@ __device__ __forceinline__ float gn_dact(float z, int act) {
   return s * (1.f + z * (1.f - s));
 }
 
-// a part's (sum, squared deviations from its own mean) joined with another's
-__device__ __forceinline__ void gn_join(float na, float& sa, float& qa, float nb, float sb, float qb) {
-  if (nb <= 0.f) return;
-  if (na <= 0.f) { sa = sb, qa = qb; return; }
-  const float d = sb / nb - sa / na;
-  qa += qb + d * d * (na * nb / (na + nb));
-  sa += sb;
-}
+// a part's (sum, squared deviations from its own mean) joined with another's: what depends on the counts alone, then a channel
+struct gn_joint {
+  float ia, ib, f;
+  __device__ __forceinline__ gn_joint(float na, float nb) : ia(na > 0.f ? 1.f / na : 0.f), ib(nb > 0.f ? 1.f / nb : 0.f), f(na > 0.f && nb > 0.f ? na * nb / (na + nb) : 0.f) {}
+  __device__ __forceinline__ void operator()(float& sa, float& qa, float sb, float qb) const {
+    const float d = sb * ib - sa * ia;
+    qa += __builtin_fmaf(d * d, f, qb);
+    sa += sb;
+  }
+};
 
 // rows k = ty, ty + ny, .. of `n` rows, at most GN_R of them
-__device__ __forceinline__ int gn_mine(int64_t n, int ty, int ny) { return n > ty ? (int)min((n - ty + ny - 1) / ny, (int64_t)GN_R) : 0; }
+__device__ __forceinline__ int gn_mine(int64_t n, int ty, int ny, int most = GN_R) { return n > ty ? (int)min((n - ty + ny - 1) / ny, (int64_t)most) : 0; }
 
 // sum and squared deviations of a thread's `mine` rows, per channel
-template <typename T, int VEC>
-__device__ __forceinline__ void gn_moments(const gn_vec<T, VEC> (&v)[GN_R], int mine, float (&s)[VEC], float (&q)[VEC]) {
+template <typename T, int VEC, int R>
+__device__ __forceinline__ void gn_moments(const gn_vec<T, VEC> (&v)[R], int mine, float (&s)[VEC], float (&q)[VEC]) {
   const float inv = mine > 0 ? 1.f / (float)mine : 0.f;
 #pragma unroll
   for (int c = 0; c < VEC; ++c) {
     s[c] = 0.f, q[c] = 0.f;
 #pragma unroll
-    for (int k = 0; k < GN_R; ++k) s[c] += k < mine ? (float)v[k].e[c] : 0.f;
+    for (int k = 0; k < R; ++k) s[c] += k < mine ? (float)v[k].e[c] : 0.f;
     const float mu = s[c] * inv;
 #pragma unroll
-    for (int k = 0; k < GN_R; ++k) {
+    for (int k = 0; k < R; ++k) {
       const float d = (float)v[k].e[c] - mu;
       q[c] += k < mine ? d * d : 0.f;
     }
@@ -105,7 +108,7 @@ __device__ __forceinline__ void gn_reduce_rows(float* s1, float* s2, float* n, f
       if constexpr (MOMENTS) na = n[ty], nb = n[ty + half];
 #pragma unroll
       for (int c = 0; c < VEC; ++c) {
-        if constexpr (MOMENTS) gn_join(na, s1[at + c], s2[at + c], nb, s1[from + c], s2[from + c]);
+        if constexpr (MOMENTS) gn_joint(na, nb)(s1[at + c], s2[at + c], s1[from + c], s2[from + c]);
         else s1[at + c] += s1[from + c], s2[at + c] += s2[from + c];
       }
     }
@@ -116,6 +119,11 @@ __device__ __forceinline__ void gn_reduce_rows(float* s1, float* s2, float* n, f
   }
   __syncthreads();
 }
+
+// Rows of a thread in the last pass.  A 4-byte type streams best in short workgroups (64 x 256 x 256 x 96: 561 us with 4 rows, 593 with 16); a
+// 2-byte type has twice the channels' coefficients to fetch first (32 x 64 x 64 x 384: 68 us with 4 rows, 45 with 16; its gradient 84 and
+// 73 with 4 and 8).
+constexpr int gn_apply_rows(int vec, bool bwd) { return vec == 8 ? (bwd ? 8 : 16) : 4; }
 
 template <int VEC>
 struct gn_coef {
@@ -129,10 +137,12 @@ struct gn_coef {
     }
   }
   __device__ __forceinline__ void stat(const GnP& p, int b, int c0) {
+    int64_t g = (int64_t)b * p.G + c0 / p.Cg;
+    int in = c0 % p.Cg;
 #pragma unroll
     for (int c = 0; c < VEC; ++c) {
-      const int64_t g = (int64_t)b * p.G + (c0 + c) / p.Cg;
       mean[c] = p.mean[g], rstd[c] = p.rstd[g];
+      if (++in == p.Cg) in = 0, ++g;
     }
   }
   __device__ __forceinline__ float z(float x, int c, float& xh) const {
@@ -164,7 +174,7 @@ __global__ __launch_bounds__(THREADS) void icg_groupnorm_slab_kernel(GnP p) {
   if (active) k_.affine(p, b, c0);
   float a[VEC], q[VEC];
   if constexpr (!BWD) {
-    gn_moments<T, VEC>(v, mine, a, q);
+    gn_moments<T, VEC, GN_R>(v, mine, a, q);
     gn_reduce_rows<VEC, true>(s1, s2, n, a, q, (float)mine, tx, ty, p.cc, p.ny, active);
     const float rows = (float)p.HW, all = rows * (float)p.Cg;
     for (int g = wv; g < groups; g += THREADS / 64) {
@@ -269,36 +279,36 @@ __global__ __launch_bounds__(256) void icg_groupnorm_part_kernel(GnP p) {
   if constexpr (BWD) {
     if (active) k_.affine(p, b, c0), k_.stat(p, b, c0);
   }
-  if (active)
-    for (int64_t s = 0; s < rows; s += (int64_t)GN_R * p.ny) {
-      const int mine = gn_mine(rows - s, ty, p.ny);
-      gn_vec<T, VEC> v[GN_R], dv[BWD ? GN_R : 1];
+  if (active) {
+    if constexpr (BWD) {
+      const T* dy = reinterpret_cast<const T*>(p.dy) + ((int64_t)b * p.HW + r0) * p.C + c0;
+      for (int64_t r = ty; r < rows; r += p.ny) {
+        const gn_vec<T, VEC> v = gn_load<T, VEC>(x + r * p.C), dv = gn_load<T, VEC>(dy + r * p.C);
 #pragma unroll
-      for (int k = 0; k < GN_R; ++k)
-        if (k < mine) {
-          const int64_t at = (s + ty + (int64_t)k * p.ny) * p.C;
-          v[k] = gn_load<T, VEC>(x + at);
-          if constexpr (BWD) dv[k] = gn_load<T, VEC>(reinterpret_cast<const T*>(p.dy) + ((int64_t)b * p.HW + r0) * p.C + c0 + at);
+        for (int c = 0; c < VEC; ++c) {
+          float xh;
+          const float z = k_.z((float)v.e[c], c, xh), dz = (float)dv.e[c] * gn_dact(z, p.act);
+          a[c] += dz;
+          q[c] = __builtin_fmaf(dz, xh, q[c]);
         }
-      if constexpr (BWD) {
+      }
+    } else {
+      for (int64_t s = 0; s < rows; s += (int64_t)GN_P * p.ny) {
+        const int mine = gn_mine(rows - s, ty, p.ny, GN_P);
+        gn_vec<T, VEC> v[GN_P];
 #pragma unroll
-        for (int k = 0; k < GN_R; ++k)
-          if (k < mine)
-#pragma unroll
-            for (int c = 0; c < VEC; ++c) {
-              float xh;
-              const float z = k_.z((float)v[k].e[c], c, xh), dz = (float)dv[k].e[c] * gn_dact(z, p.act);
-              a[c] += dz;
-              q[c] = __builtin_fmaf(dz, xh, q[c]);
-            }
-      } else if (mine > 0) {
+        for (int k = 0; k < GN_P; ++k)
+          if (k < mine) v[k] = gn_load<T, VEC>(x + (s + ty + (int64_t)k * p.ny) * p.C);
+        if (mine == 0) continue;
         float sa[VEC], qa[VEC];
-        gn_moments<T, VEC>(v, mine, sa, qa);
+        gn_moments<T, VEC, GN_P>(v, mine, sa, qa);
+        const gn_joint join(count, (float)mine);
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) gn_join(count, a[c], q[c], (float)mine, sa[c], qa[c]);
+        for (int c = 0; c < VEC; ++c) join(a[c], q[c], sa[c], qa[c]);
         count += (float)mine;
       }
     }
+  }
   gn_reduce_rows<VEC, !BWD>(s1, s2, n, a, q, count, tx, ty, p.cc, p.ny, active);
   float* out = p.part + ((int64_t)b * p.nchunks + blockIdx.x) * 2 * p.C;
   for (int c = tid; c < p.cc * VEC; c += 256) {
@@ -358,31 +368,33 @@ __global__ __launch_bounds__(256) void icg_groupnorm_join_bwd_kernel(GnP p, floa
   if (threadIdx.x == 0) coef[2 * blockIdx.x] = (float)(u / all), coef[2 * blockIdx.x + 1] = (float)(w / all);
 }
 
-// ---- third: y, or dx
+// ---- third: y, or dx.  Blocks run from the end of the tensor: what the first pass read last may still be in the caches.
 template <typename T, int VEC, bool BWD>
-__global__ __launch_bounds__(256) void icg_groupnorm_apply_kernel(GnP p, const float* coef) {
+__global__ __launch_bounds__(256) void icg_groupnorm_apply_kernel(GnP p, const float* coef, int per_block) {
   const int tid = threadIdx.x, tx = tid % p.cc, ty = tid / p.cc;
-  const int c0 = (blockIdx.y * p.cc + tx) * VEC, b = blockIdx.z;
+  const int c0 = (blockIdx.y * p.cc + tx) * VEC, b = p.B - 1 - blockIdx.z;
   if (ty >= p.ny || c0 >= p.C) return;
-  const int64_t r0 = (int64_t)blockIdx.x * p.rows, rows = min(p.rows, p.HW - r0);
-  const int64_t base = ((int64_t)b * p.HW + r0) * p.C + c0;
+  const int64_t r0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * per_block, rows = min((int64_t)per_block, p.HW - r0), base = ((int64_t)b * p.HW + r0) * p.C + c0;
   const T* x = reinterpret_cast<const T*>(p.x) + base;
+  const T* dy = reinterpret_cast<const T*>(p.dy) + (BWD ? base : 0);
   T* out = reinterpret_cast<T*>(BWD ? p.dx : p.y) + base;
   gn_coef<VEC> k_;
   k_.affine(p, b, c0);
   k_.stat(p, b, c0);
   float m1[VEC], m2[VEC];
   if constexpr (BWD) {
+    int64_t g = (int64_t)b * p.G + c0 / p.Cg;
+    int in = c0 % p.Cg;
 #pragma unroll
     for (int c = 0; c < VEC; ++c) {
-      const int64_t g = (int64_t)b * p.G + (c0 + c) / p.Cg;
       m1[c] = coef[2 * g], m2[c] = coef[2 * g + 1];
+      if (++in == p.Cg) in = 0, ++g;
     }
   }
   for (int64_t r = ty; r < rows; r += p.ny) {
     const gn_vec<T, VEC> v = gn_load<T, VEC>(x + r * p.C);
-    gn_vec<T, VEC> o, dv;
-    if constexpr (BWD) dv = gn_load<T, VEC>(reinterpret_cast<const T*>(p.dy) + base + r * p.C);
+    gn_vec<T, VEC> dv, o;
+    if constexpr (BWD) dv = gn_load<T, VEC>(dy + r * p.C);
 #pragma unroll
     for (int c = 0; c < VEC; ++c) {
       float xh;
@@ -403,6 +415,7 @@ __global__ __launch_bounds__(256) void icg_groupnorm_batch_sum_kernel(const floa
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= C) return;
   double g = 0.0, s = 0.0;
+#pragma unroll 8
   for (int b = 0; b < B; ++b) g += dgain_b[(int64_t)b * C + c], s += dbias_b[(int64_t)b * C + c];
   dgain[c] = (float)g, dbias[c] = (float)s;
 }
@@ -419,7 +432,7 @@ bool gn_shape_ok(int B, int64_t HW, int C, int G, int dtype) {
   return B > 0 && B < 65536 && HW > 0 && HW < (1LL << 30) && C > 0 && C < (1 << 20) && G > 0 && C % G == 0 && dtype >= 0 && dtype <= 2 && (int64_t)B * G < 0x7fffffffL;
 }
 
-GnPlan gn_plan(int B, int64_t HW, int C, int G, int dtype, bool vec) {
+GnPlan gn_plan(int B, int64_t HW, int C, int G, int dtype, bool vec, bool bwd) {
   GnPlan pl = {};
   const int per = dtype == 0 ? 4 : 8, v = vec && C % per == 0 ? per : 1, Cg = C / G;
   pl.vec = v > 1;
@@ -428,7 +441,8 @@ GnPlan gn_plan(int B, int64_t HW, int C, int G, int dtype, bool vec) {
   int gs = 1;
   while (gs <= G && (G % gs != 0 || (gs * Cg) % v != 0)) ++gs;
   auto fits = [&](int set, int threads) { const int cc = set * Cg / v; return cc <= threads && HW <= (int64_t)(threads / cc) * GN_R; };
-  if (gs <= G && (fits(gs, 256) || fits(gs, 1024))) {
+  const bool wide = !(bwd && v == 8);                      // (1024 threads have 128 registers each: too few for 8 rows of x and dy in 16 bits)
+  if (gs <= G && (fits(gs, 256) || (wide && fits(gs, 1024)))) {
     pl.slab = true;
     while (G % (2 * gs) == 0 && fits(2 * gs, 256) && (int64_t)B * (G / (2 * gs)) >= 512) gs *= 2;
     pl.threads = fits(gs, 256) ? 256 : 1024;
@@ -445,10 +459,11 @@ GnPlan gn_plan(int B, int64_t HW, int C, int G, int dtype, bool vec) {
     const double used = (double)cv / ((double)n * cc) * ny * cc / 256.0;
     if (used > best + 1e-9) best = used, pl.cc = cc, pl.ncol = (int)icg_cdiv(cv, cc), pl.ny = ny;
   }
-  // chunks of whole register batches; no more workgroups than 16 for each compute unit
-  const int64_t batch = (int64_t)pl.ny * GN_R;
+  // chunks of whole batches; 4 workgroups for each compute unit, 8 in the gradient (64 x 256 x 256 x 96 fp32: 314 us with 4, 360 with 8, 333 with
+  // 16; the gradient of 32 x 64 x 64 x 384 bf16: 54, 47, 57)
+  const int64_t batch = (int64_t)pl.ny * GN_P;
   int64_t chunks = icg_cdiv(HW, batch);
-  const int64_t most = icg_cdiv(16 * 256, (int64_t)B * pl.ncol);
+  const int64_t most = icg_cdiv((bwd ? 8 : 4) * 256, (int64_t)B * pl.ncol);
   if (chunks > most) chunks = most;
   pl.rows = icg_cdiv(icg_cdiv(HW, chunks), batch) * batch;
   pl.nchunks = (int)icg_cdiv(HW, pl.rows);
@@ -456,10 +471,10 @@ GnPlan gn_plan(int B, int64_t HW, int C, int G, int dtype, bool vec) {
 }
 
 // (the plan with 16-byte columns and the one without differ in their chunks: room for either)
-size_t gn_part_bytes(int B, int64_t HW, int C, int G, int dtype) {
+size_t gn_part_bytes(int B, int64_t HW, int C, int G, int dtype, bool bwd) {
   size_t most = 0;
   for (int vec = 0; vec < 2; ++vec) {
-    const GnPlan pl = gn_plan(B, HW, C, G, dtype, vec != 0);
+    const GnPlan pl = gn_plan(B, HW, C, G, dtype, vec != 0, bwd);
     const size_t n = pl.slab ? 0 : (size_t)B * pl.nchunks * 2 * C * 4 + (size_t)B * G * 2 * 4;
     if (n > most) most = n;
   }
@@ -488,7 +503,9 @@ int gn_run(const GnPlan& pl, const GnP& p, hipStream_t st) {
   if (BWD) hipLaunchKernelGGL(icg_groupnorm_join_bwd_kernel, dim3((unsigned)(p.B * p.G)), dim3(256), 0, st, p, coef);
   else hipLaunchKernelGGL(icg_groupnorm_join_kernel, dim3((unsigned)(p.B * p.G)), dim3(256), 0, st, p);
   if (const int e = icg_check_launch()) return e;
-  hipLaunchKernelGGL((icg_groupnorm_apply_kernel<T, VEC, BWD>), grid, dim3(256), 0, st, p, (const float*)coef);
+  const int per_block = p.ny * gn_apply_rows(VEC, BWD);
+  const dim3 apply((unsigned)icg_cdiv(p.HW, per_block), (unsigned)pl.ncol, (unsigned)p.B);
+  hipLaunchKernelGGL((icg_groupnorm_apply_kernel<T, VEC, BWD>), apply, dim3(256), 0, st, p, (const float*)coef, per_block);
   return icg_check_launch();
 }
 
@@ -502,7 +519,7 @@ int gn_dispatch(const GnPlan& pl, const GnP& p, int dtype, hipStream_t st) {
 }  // namespace
 
 extern "C" size_t icg_groupnorm_fwd_workspace_bytes(int B, int64_t HW, int C, int G, int dtype) {
-  return gn_shape_ok(B, HW, C, G, dtype) ? gn_part_bytes(B, HW, C, G, dtype) : 0;
+  return gn_shape_ok(B, HW, C, G, dtype) ? gn_part_bytes(B, HW, C, G, dtype, false) : 0;
 }
 
 extern "C" int icg_groupnorm_act_fwd(const void* x, const float* gain, const float* bias, void* y, float* mean, float* rstd, int B, int64_t HW, int C,
@@ -510,12 +527,12 @@ extern "C" int icg_groupnorm_act_fwd(const void* x, const float* gain, const flo
                                      void* stream) {
   ICG_REQUIRE(x && y && mean && rstd && gn_shape_ok(B, HW, C, G, dtype) && act >= 0 && act <= 2 && eps >= 0.f && eps < INFINITY);
   const bool vec = ((uintptr_t)x % 16) == 0 && ((uintptr_t)y % 16) == 0;
-  const GnPlan pl = gn_plan(B, HW, C, G, dtype, vec);
+  const GnPlan pl = gn_plan(B, HW, C, G, dtype, vec, false);
   ICG_REQUIRE((int64_t)B * pl.ncol < 0x7fffffffL && pl.ncol < 65536);
   GnP p = gn_params(pl, B, HW, C, G, per_sample, gain_offset, eps, act);
   p.x = x, p.gain = gain, p.bias = bias, p.y = y, p.mean = mean, p.rstd = rstd;
   if (!pl.slab) {
-    if (workspace_bytes < gn_part_bytes(B, HW, C, G, dtype)) return ICG_ERR_WORKSPACE;
+    if (workspace_bytes < gn_part_bytes(B, HW, C, G, dtype, false)) return ICG_ERR_WORKSPACE;
     ICG_REQUIRE(workspace && ((uintptr_t)workspace % 16) == 0);
     p.part = (float*)workspace;
   }
@@ -523,7 +540,7 @@ extern "C" int icg_groupnorm_act_fwd(const void* x, const float* gain, const flo
 }
 
 extern "C" size_t icg_groupnorm_bwd_workspace_bytes(int B, int64_t HW, int C, int G, int dtype) {
-  return gn_shape_ok(B, HW, C, G, dtype) ? gn_part_bytes(B, HW, C, G, dtype) + (size_t)B * C * 2 * 4 : 0;
+  return gn_shape_ok(B, HW, C, G, dtype) ? gn_part_bytes(B, HW, C, G, dtype, true) + (size_t)B * C * 2 * 4 : 0;
 }
 
 extern "C" int icg_groupnorm_act_bwd(const void* x, const void* dy, const float* gain, const float* bias, const float* mean, const float* rstd, void* dx,
@@ -533,12 +550,12 @@ extern "C" int icg_groupnorm_act_bwd(const void* x, const void* dy, const float*
   if (workspace_bytes < icg_groupnorm_bwd_workspace_bytes(B, HW, C, G, dtype)) return ICG_ERR_WORKSPACE;
   ICG_REQUIRE(workspace && ((uintptr_t)workspace % 16) == 0);
   const bool vec = ((uintptr_t)x % 16) == 0 && ((uintptr_t)dy % 16) == 0 && ((uintptr_t)dx % 16) == 0;
-  const GnPlan pl = gn_plan(B, HW, C, G, dtype, vec);
+  const GnPlan pl = gn_plan(B, HW, C, G, dtype, vec, true);
   ICG_REQUIRE((int64_t)B * pl.ncol < 0x7fffffffL && pl.ncol < 65536);
   GnP p = gn_params(pl, B, HW, C, G, per_sample, gain_offset, eps, act);
   p.x = x, p.dy = dy, p.gain = gain, p.bias = bias, p.dx = dx, p.mean = const_cast<float*>(mean), p.rstd = const_cast<float*>(rstd);
   p.part = (float*)workspace;
-  float* sums = (float*)((char*)workspace + gn_part_bytes(B, HW, C, G, dtype));
+  float* sums = (float*)((char*)workspace + gn_part_bytes(B, HW, C, G, dtype, true));
   const bool shared = dgain && !per_sample;
   p.dgain = shared ? sums : dgain, p.dbias = shared ? sums + (size_t)B * C : dbias;
   if (const int e = gn_dispatch<true>(pl, p, dtype, (hipStream_t)stream)) return e;
