@@ -22,10 +22,7 @@ struct EmbP {
   float* part;                        // [ceil(n / EMB_CHUNK)][2][D]
 };
 
-#ifndef EMB_C
-#define EMB_C 32
-#endif
-constexpr int EMB_CHUNK = EMB_C;         // list entries of one piece
+constexpr int EMB_CHUNK = 32;         // list entries of one piece
 constexpr int EMB_RUN = 1024;         // most tokens a workgroup of the sort owns (64 KB of counts)
 constexpr int EMB_FEW = 1024;         // up to here the gradient scans the list per row, in one launch
 
@@ -109,7 +106,7 @@ __global__ __launch_bounds__(256) void icg_embedding_bwd_few_kernel(EmbP p) {
 }
 
 // ---- the positions in the order of their tokens
-constexpr int EMB_WAVES = 16, EMB_BATCH = 8;
+constexpr int EMB_WAVES = 16, EMB_KEEP = 16;
 __global__ __launch_bounds__(64 * EMB_WAVES) void icg_embedding_sort_kernel(EmbP p) {
   __shared__ int count[EMB_WAVES * EMB_RUN];               // [wave][token]: occurrences, then the next place
   __shared__ int less[EMB_WAVES], sums[EMB_WAVES];
@@ -120,27 +117,29 @@ __global__ __launch_bounds__(64 * EMB_WAVES) void icg_embedding_sort_kernel(EmbP
   __syncthreads();
   const int64_t share = (p.n + EMB_WAVES * 64 - 1) / (EMB_WAVES * 64) * 64, i0 = wv * share, i1 = min(i0 + share, p.n);
   int below = 0;
-  // (EMB_BATCH loads in flight: a sweep waits for its list, not for its arithmetic)
-  for (int64_t g = i0; g < i1; g += 64 * EMB_BATCH) {
-    int64_t ahead[EMB_BATCH];
-#pragma unroll
-    for (int k = 0; k < EMB_BATCH; ++k) ahead[k] = g + 64 * k + lane < i1 ? em_token(p, g + 64 * k + lane) : -1;
-#pragma unroll
-    for (int k = 0; k < EMB_BATCH; ++k) {
-    const int64_t t = ahead[k];
+  // a token of this workgroup's run, or -1
+  auto local = [&](int64_t i) -> int {
+    const int64_t t = i < i1 ? em_token(p, i) : -1;
     const bool valid = (uint64_t)t < (uint64_t)p.V && t != p.pad;
     below += __builtin_popcountll(__ballot(valid && t < v0));
-    const int u = valid && t >= v0 && t < v0 + own ? (int)(t - v0) : -1;
+    return valid && t >= v0 && t < v0 + own ? (int)(t - v0) : -1;
+  };
+  auto tally = [&](int u) {
     unsigned long long rest = __ballot(u >= 0);
     while (rest) {                                         // one distinct token at a time
       const int first = __builtin_ctzll(rest);
-      const unsigned long long same = __ballot(u == __shfl(u, first, 64));
+      const unsigned long long same = __ballot(u == __builtin_amdgcn_readlane(u, first));
       if (lane == first) count[wv * p.run + u] += __builtin_popcountll(same);
       rest &= ~same;
     }
     icg_wave_lds_sync();
-    }
-  }
+  };
+  int kept[EMB_KEEP];                                      // the share's first tokens stay in registers for the second sweep
+#pragma unroll
+  for (int k = 0; k < EMB_KEEP; ++k) kept[k] = i0 + 64 * k < i1 ? local(i0 + 64 * k + lane) : -1;
+#pragma unroll
+  for (int k = 0; k < EMB_KEEP; ++k) tally(kept[k]);
+  for (int64_t i = i0 + 64 * EMB_KEEP; i < i1; i += 64) tally(local(i + lane));
   if (lane == 0) less[wv] = below;
   __syncthreads();
   // places: tokens in order, and within a token the waves in order.  Thread t takes token t (run <= 1024 = the threads).
@@ -171,30 +170,24 @@ __global__ __launch_bounds__(64 * EMB_WAVES) void icg_embedding_sort_kernel(EmbP
     if (v0 + tid == p.V - 1) p.start[p.V] = next;
   }
   __syncthreads();
-  for (int64_t g = i0; g < i1; g += 64 * EMB_BATCH) {
-    int64_t ahead[EMB_BATCH];
-#pragma unroll
-    for (int k = 0; k < EMB_BATCH; ++k) ahead[k] = g + 64 * k + lane < i1 ? em_token(p, g + 64 * k + lane) : -1;
-#pragma unroll
-    for (int k = 0; k < EMB_BATCH; ++k) {
-    const int64_t i = g + 64 * k, t = ahead[k];
-    const bool hit = t >= v0 && t < v0 + own && t != p.pad;
-    const int u = hit ? (int)(t - v0) : -1;
-    unsigned long long rest = __ballot(hit);
+  auto place = [&](int64_t i, int u) {
+    unsigned long long rest = __ballot(u >= 0);
     while (rest) {                                         // one distinct token at a time, its entries in lane order
       const int first = __builtin_ctzll(rest);
-      const int tok = __shfl(u, first, 64);
+      const int tok = __builtin_amdgcn_readlane(u, first);
       const unsigned long long same = __ballot(u == tok);
       int* next = &count[wv * p.run + tok];
-      const int place = *next;
+      const int at = *next;
       icg_wave_lds_sync();
-      if (u == tok) p.order[place + __builtin_popcountll(same & ((1ull << lane) - 1))] = (int)(i + lane);
-      if (lane == first) *next = place + __builtin_popcountll(same);
+      if (u == tok) p.order[at + __builtin_popcountll(same & ((1ull << lane) - 1))] = (int)(i + lane);
+      if (lane == first) *next = at + __builtin_popcountll(same);
       icg_wave_lds_sync();
       rest &= ~same;
     }
-    }
-  }
+  };
+#pragma unroll
+  for (int k = 0; k < EMB_KEEP; ++k) place(i0 + 64 * k, kept[k]);
+  for (int64_t i = i0 + 64 * EMB_KEEP; i < i1; i += 64) place(i, local(i + lane));
 }
 
 // a token that fills more than a piece: the sum of its entries in piece k is part[k][0] if it began in an earlier piece, else part[k][1]
@@ -207,95 +200,70 @@ __global__ __launch_bounds__(64) void icg_embedding_bwd_piece_kernel(EmbP p) {
   if (e0 >= total) return;
   const int lane = threadIdx.x;
   const int64_t c = (int64_t)blockIdx.y * 64 * VEC + lane * VEC;
+  const int side = blockIdx.z;
+  const int64_t t = em_token(p, p.order[side == 0 ? e0 : e1 - 1]);
+  const int b = p.start[t], e = p.start[t + 1];
+  if (e - b <= EMB_CHUNK || (side == 0) != (b < e0) || c >= p.D) return;
+  float a[VEC];
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const int64_t t = em_token(p, p.order[side == 0 ? e0 : e1 - 1]);
-    const int b = p.start[t], e = p.start[t + 1];
-    if (e - b <= EMB_CHUNK || (side == 0) != (b < e0)) continue;
-    if (c >= p.D) continue;
-    float a[VEC];
+  for (int j = 0; j < VEC; ++j) a[j] = 0.f;
+  int i = max(b, e0);
+  const int to = min(e, e1);
+  for (; i + 8 <= to; i += 8) {
+    em_vec<T, VEC> v[8];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) a[j] = 0.f;
-    const int from = max(b, e0), to = min(e, e1);
-    int i = from;
-    for (; i + 8 <= to; i += 8) {
-      em_vec<T, VEC> v[8];
+    for (int q = 0; q < 8; ++q) v[q] = em_load<T, VEC>(reinterpret_cast<const T*>(p.dout) + (int64_t)p.order[i + q] * p.D + c);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = em_load<T, VEC>(reinterpret_cast<const T*>(p.dout) + (int64_t)p.order[i + q] * p.D + c);
+    for (int q = 0; q < 8; ++q)
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) a[j] += (float)v[q].e[j];
-    }
-    for (; i < to; ++i) em_add<T, VEC>(a, p, p.order[i], c);
-    float* out = p.part + (k * 2 + side) * p.D + c;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) out[j] = a[j];
+      for (int j = 0; j < VEC; ++j) a[j] += (float)v[q].e[j];
   }
+  for (; i < to; ++i) em_add<T, VEC>(a, p, p.order[i], c);
+  float* out = p.part + (k * 2 + side) * p.D + c;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) out[j] = a[j];
 }
 
-// a wave per row of the table, EMB_TILES column tiles at once so that an entry's whole row is in flight
-constexpr int EMB_TILES = 4;
+// a wave per column tile of a row of the table: the longest piece of work is a tile of EMB_CHUNK entries, or of one sum per EMB_CHUNK entries
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void icg_embedding_bwd_row_kernel(EmbP p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (v >= p.V) return;
+__global__ __launch_bounds__(256) void icg_embedding_bwd_row_kernel(EmbP p, int tiles) {
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), v = w / tiles, c = ((w - v * tiles) * 64 + (threadIdx.x & 63)) * VEC;
+  if (v >= p.V || c >= p.D) return;
   const int b = p.start[v], e = p.start[v + 1];
-  for (int64_t c0 = lane * VEC; c0 < p.D; c0 += 64 * VEC * EMB_TILES) {
-    float a[EMB_TILES][VEC];
+  float a[VEC];
 #pragma unroll
-    for (int u = 0; u < EMB_TILES; ++u)
+  for (int j = 0; j < VEC; ++j) a[j] = 0.f;
+  if (e - b <= EMB_CHUNK) {
+    const T* dout = reinterpret_cast<const T*>(p.dout) + c;
+    int i = b;
+    for (; i + 4 <= e; i += 4) {
+      em_vec<T, VEC> x[4];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) a[u][j] = 0.f;
-    if (e - b <= EMB_CHUNK) {
-      const T* dout = reinterpret_cast<const T*>(p.dout) + c0;
-      int i = b;
-      for (; i + 2 <= e; i += 2) {
-        em_vec<T, VEC> x[2][EMB_TILES];
+      for (int q = 0; q < 4; ++q) x[q] = em_load<T, VEC>(dout + (int64_t)p.order[i + q] * p.D);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const T* row = dout + (int64_t)p.order[i + q] * p.D;
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int u = 0; u < EMB_TILES; ++u)
-            if (c0 + u * 64 * VEC < p.D) x[q][u] = em_load<T, VEC>(row + u * 64 * VEC);
-        }
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-          for (int u = 0; u < EMB_TILES; ++u)
-            if (c0 + u * 64 * VEC < p.D)
-#pragma unroll
-              for (int j = 0; j < VEC; ++j) a[u][j] += (float)x[q][u].e[j];
-      }
-      if (i < e)
-#pragma unroll
-        for (int u = 0; u < EMB_TILES; ++u)
-          if (c0 + u * 64 * VEC < p.D) em_add<T, VEC>(a[u], p, p.order[i], c0 + u * 64 * VEC);
-    } else {
-      const int k0 = b / EMB_CHUNK, k1 = (e - 1) / EMB_CHUNK;
-#pragma unroll
-      for (int u = 0; u < EMB_TILES; ++u) {
-        if (c0 + u * 64 * VEC >= p.D) continue;
-        const float* in = p.part + c0 + u * 64 * VEC;
-#pragma unroll 4
-        for (int k = k0; k <= k1; ++k) {
-          const float* q = in + ((int64_t)k * 2 + (b < k * EMB_CHUNK ? 0 : 1)) * p.D;
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) a[u][j] += q[j];
-        }
-      }
+        for (int j = 0; j < VEC; ++j) a[j] += (float)x[q].e[j];
     }
+    for (; i < e; ++i) em_add<T, VEC>(a, p, p.order[i], c);
+  } else {
+    const int k0 = b / EMB_CHUNK, k1 = (e - 1) / EMB_CHUNK;
+    const float* in = p.part + c;
+#pragma unroll 4
+    for (int k = k0; k <= k1; ++k) {
+      const float* q = in + ((int64_t)k * 2 + (b < k * EMB_CHUNK ? 0 : 1)) * p.D;
 #pragma unroll
-    for (int u = 0; u < EMB_TILES; ++u)
-      if (c0 + u * 64 * VEC < p.D) em_write<T, VEC>(a[u], p, v, c0 + u * 64 * VEC);
+      for (int j = 0; j < VEC; ++j) a[j] += q[j];
+    }
   }
+  em_write<T, VEC>(a, p, v, c);
 }
 
 namespace {
 
+// (column tiles of 64 elements at the narrowest are a grid's second dimension: at most 32768 of them)
 bool em_shape_ok(int64_t n, int64_t V, int64_t D, int dtype) {
-  return n > 0 && n < 0x7fffff00LL && V > 0 && V < 0x7fffff00LL && D > 0 && D < (1 << 24) && dtype >= 0 && dtype <= 2;
+  return n > 0 && n < 0x7fffff00LL && V > 0 && V < 0x7fffff00LL && D > 0 && D < (1 << 21) && dtype >= 0 && dtype <= 2;
 }
 size_t em_align(size_t x) { return (x + 15) / 16 * 16; }
 
@@ -316,9 +284,11 @@ int em_bwd(const EmbP& p, hipStream_t st) {
   }
   hipLaunchKernelGGL(icg_embedding_sort_kernel, dim3((unsigned)icg_cdiv(p.V, p.run)), dim3(64 * EMB_WAVES), 0, st, p);
   if (const int e = icg_check_launch()) return e;
-  hipLaunchKernelGGL((icg_embedding_bwd_piece_kernel<T, VEC>), dim3((unsigned)icg_cdiv(p.n, EMB_CHUNK), (unsigned)icg_cdiv(p.D, 64 * VEC)), dim3(64), 0, st, p);
+  hipLaunchKernelGGL((icg_embedding_bwd_piece_kernel<T, VEC>), dim3((unsigned)icg_cdiv(p.n, EMB_CHUNK), (unsigned)icg_cdiv(p.D, 64 * VEC), 2), dim3(64), 0, st, p);
   if (const int e = icg_check_launch()) return e;
-  hipLaunchKernelGGL((icg_embedding_bwd_row_kernel<T, VEC>), dim3(rows), dim3(256), 0, st, p);
+  const int64_t tiles = icg_cdiv(p.D, 64 * VEC), blocks = icg_cdiv(p.V * tiles, 4);
+  ICG_REQUIRE(blocks < 0x7fffffffLL);
+  hipLaunchKernelGGL((icg_embedding_bwd_row_kernel<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, p, (int)tiles);
   return icg_check_launch();
 }
 
@@ -353,8 +323,8 @@ extern "C" int icg_embedding_bwd(const void* idx, const void* dout, void* dweigh
     p.order = (int*)at, at += em_align((size_t)n * 4);
     p.start = (int*)at, at += em_align((size_t)(V + 1) * 4);
     p.part = (float*)at;
-    // two workgroups for each compute unit, within the counts that fit
-    const int64_t run = icg_cdiv(V, 512);
+    // a workgroup for each compute unit, within the counts that fit (each reads the whole list: fewer read less)
+    const int64_t run = icg_cdiv(V, 256);
     p.run = (int)(run < EMB_RUN ? run : EMB_RUN);
   }
   const bool al = ((uintptr_t)dweight % 16) == 0 && ((uintptr_t)dout % 16) == 0;

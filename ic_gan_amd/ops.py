@@ -1414,7 +1414,7 @@ def attention(q, k, v, *, scale=None, causal=False, k_lens=None, q_start=None, r
     k_lens     [B]: sequence b has its first k_lens[b] keys only (held to 0 .. Lk); what lies behind them is never read
     causal     query i of sequence b sees keys up to q_start[b] + i
     q_start    [B], default Lk - Lq: the position of the sequence's first query among the keys (used when causal)
-    A query that sees no key gets zeros, -inf and no gradient.  One or few queries (a token at a time against a cache) take a kernel that
+    A query that sees no key (or whose scores are all -inf) gets zeros, -inf and no gradient.  One or few queries (a token at a time against a cache) take a kernel that
     splits the keys over the chip."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not isinstance(t, torch.Tensor) or t.dim() != 4:
@@ -1580,7 +1580,7 @@ def embedding(idx, weight, *, scale=1.0, padding_idx=None):
     if idx.device != weight.device:
         raise ValueError("embedding: idx is on %s, weight on %s" % (idx.device, weight.device))
     V, D = weight.shape
-    if V == 0 or D == 0 or D >= 1 << 24 or max(V, idx.numel()) >= 0x7fffff00:
+    if V == 0 or D == 0 or D >= 1 << 21 or max(V, idx.numel()) >= 0x7fffff00:
         raise ValueError("embedding: not served: table [%d, %d], %d tokens" % (V, D, idx.numel()))
     if not abs(float(scale)) < float("inf"):
         raise ValueError("embedding: scale must be finite, not %r" % scale)

@@ -6,6 +6,8 @@ step w = 2^-24):
                             times the sum of their magnitudes; the exponent's argument by a few w times its magnitude
   p, ds as operands         rounded to the element type (u relative; fp16 also 2^-25 absolute in its own scale), not at all in fp32
   D_i = do_i . o_i          from the rounded o: off by |do_i| . (bound of o_i)
+  underflow                 2^x ends at fp32's smallest normal number, f = 2^-126 (what is below becomes 0), and so do operands and sums of the
+                            matrix products: p is off by up to f beside its relative error, ds by f (1 + |dp| + |D|), a sum of n products by n f
   outputs                   one rounding to the element type"""
 import math
 
@@ -100,7 +102,7 @@ def reference(case, dtype, q, k, v, do, scale=None):
     shared = lambda t: t.view(B, Hk, G, Lk, -1).sum(2)
     dq, dk, dv_ = ds @ K * scale, shared(ds.transpose(-1, -2) @ Q * scale), shared(p.transpose(-1, -2) @ dO)
 
-    w, u = 2.0 ** -24, torch.finfo(dtype).eps / 2
+    w, u, f = 2.0 ** -24, torch.finfo(dtype).eps / 2, 2.0 ** -126
     up = 0.0 if dtype == torch.float32 else u                            # p and ds as operands
     S = (Q.abs() @ K.abs().transpose(-1, -2) * scale).masked_fill(~m, 0.0)
     biggest = lambda t: float(t.masked_fill(~torch.isfinite(t), 0.0).abs().max()) if t.numel() else 0.0
@@ -108,19 +110,19 @@ def reference(case, dtype, q, k, v, do, scale=None):
     f16 = dtype == torch.float16
     A = p @ V.abs()
     seen_v = m.double() @ V.abs()
-    b_o = (up + 2 * e) * A + (2.0 ** -25 * seen_v if f16 else 0.0) + u * o.abs()
+    b_o = (up + 2 * e) * A + ((2.0 ** -25 if f16 else 0.0) + f) * seen_v + Lk * f + u * o.abs()
     b_lse = torch.full_like(lse, e) + w * 4 * lse.abs().nan_to_num(posinf=0.0)
     aO, aQ, aK = dO.abs(), Q.abs(), K.abs()
     pT = p.transpose(-1, -2)
     mT = m.double().transpose(-1, -2)
-    b_dv = (up + e) * (pT @ aO) + (2.0 ** -31 * (mT @ aO) if f16 else 0.0)
+    b_dv = (up + e) * (pT @ aO) + ((2.0 ** -31 if f16 else 0.0) + f) * (mT @ aO) + Lq * G * f
     e_dp = w * (dv + 2) * (aO @ V.abs().transpose(-1, -2))
     e_D = (aO * b_o).sum(-1, keepdim=True) + w * (dv + 2) * (aO * o.abs()).sum(-1, keepdim=True)
-    E = p * (e_dp + e_D) + (up + e) * ds.abs() + e * p * (dp.abs() + D.abs())
+    E = p * (e_dp + e_D) + (up + e) * ds.abs() + e * p * (dp.abs() + D.abs()) + f * m.double() * (1 + dp.abs() + D.abs())
     if f16:                                                              # ds is held 2^6 / (2^k, the largest |do| of what is summed) times as large
         E = E + 2.0 ** -30 * dO.norm(dim=-1).amax() * m.double()
-    b_dq = E @ aK * scale + w * (Lk + 4) * (ds.abs() @ aK) * scale
-    b_dk = E.transpose(-1, -2) @ aQ * scale + w * (Lq * G + 4) * (ds.abs().transpose(-1, -2) @ aQ) * scale
+    b_dq = E @ aK * scale + w * (Lk + 4) * (ds.abs() @ aK) * scale + Lk * f
+    b_dk = E.transpose(-1, -2) @ aQ * scale + w * (Lq * G + 4) * (ds.abs().transpose(-1, -2) @ aQ) * scale + Lq * G * f
     back = lambda t: t.transpose(1, 2)
     tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2          # outputs that are subnormal in the type
     out = {"o": (back(o), back(b_o) + tiny), "lse": (lse, b_lse), "dq": (back(dq), back(b_dq + u * dq.abs()) + tiny)}

@@ -1,0 +1,265 @@
+"""ops.attention, ops.group_norm_act and ops.embedding as programs run them: captured and replayed, on other streams, two at once, with poisoned
+buffers, at extreme values and far addresses."""
+import pytest
+import torch
+
+from tests import attention_cases as A, norm_embedding_cases as C
+
+pytestmark = pytest.mark.gpu
+
+
+def _attention_pass(seed, dtype=torch.bfloat16, case=A.CASES[A.IDS.index("causal_padded_shifted")]):
+    from ic_gan_amd import ops
+    q, k, v, do, lens, start = A.make(case, dtype, "cuda", seed)
+    ins = [q, k, v, do]
+
+    def run(q, k, v, do):
+        o = ops.attention(q, k, v, causal=case[8], k_lens=lens, q_start=start)
+        return (o,) + torch.autograd.grad(o, (q, k, v), do)
+    return ins, run
+
+
+def _token_pass(seed, dtype=torch.float16, case=A.CASES[A.IDS.index("token_grouped_split")]):
+    from ic_gan_amd import ops
+    q, k, v, _, lens, _ = A.make(case, dtype, "cuda", seed)
+    return [t.detach() for t in (q, k, v)], lambda q, k, v: ops.attention(q, k, v, k_lens=lens, return_lse=True)
+
+
+def _norm_pass(name):
+    def make(seed, dtype=torch.bfloat16):
+        from ic_gan_amd import ops
+        case = C.NORM_CASES[C.NORM_IDS.index(name)]
+        x, dy, gain, bias = C.make_norm(case, dtype, "cuda", seed)
+
+        def run(x, dy, gain, bias):
+            y = ops.group_norm_act(x, case[5], gain, bias, act=case[6], gain_offset=case[9])
+            return (y,) + torch.autograd.grad(y, (x, gain, bias), dy)
+        return [x, dy, gain, bias], run
+    return make
+
+
+def _embedding_pass(name):
+    def make(seed, dtype=torch.float32):
+        from ic_gan_amd import ops
+        case = C.EMBEDDING_CASES[C.EMBEDDING_IDS.index(name)]
+        idx, weight, dout = C.make_embedding(case, dtype, "cuda")
+        idx = idx.roll(seed)
+
+        def run(idx, weight, dout):
+            out = ops.embedding(idx, weight, scale=case[5], padding_idx=case[6])
+            return (out,) + torch.autograd.grad(out, (weight,), dout)
+        return [idx, weight, dout], run
+    return make
+
+
+PASSES = {"attention": _attention_pass, "token": _token_pass, "norm_slab": _norm_pass("first_block"), "norm_three": _norm_pass("three_passes"),
+          "embedding_few": _embedding_pass("classes"), "embedding_sorted": _embedding_pass("sorted_padded")}
+
+
+def _same(a, b):
+    assert len(a) == len(b)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("name", PASSES)
+def test_captured_and_replayed(name):
+    """forward and backward captured into a graph: every replay, with new inputs and eager work between the replays, gives the eager bits"""
+    ins, run = PASSES[name](0)
+    more = [[t.detach().clone() for t in PASSES[name](s)[0]] for s in (1, 2, 3)]
+    eager = []
+    for new in more:
+        fresh = [t.clone().requires_grad_(old.requires_grad) for t, old in zip(new, ins)]
+        eager.append([t.detach().clone() for t in run(*fresh)])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(*ins)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(*ins)
+    for _ in range(2):
+        for new, want in zip(more, eager):
+            with torch.no_grad():
+                for t, x in zip(ins, new):
+                    t.copy_(x)
+            graph.replay()
+            torch.cuda.synchronize()
+            _same(out, want)
+            junk = torch.randn(1 << 20, device="cuda").sort().values                # eager work between the replays
+            del junk
+
+
+def test_two_graphs_at_once():
+    """two captures of the same call keep their own workspaces"""
+    graphs = []
+    for seed in (0, 1):
+        ins, run = _token_pass(seed)
+        want = [t.clone() for t in run(*ins)]
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run(*ins)
+        graphs.append((g, out, want, ins, run))              # (the graph reads the inputs' memory: they have to live on)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for (g, *_), s in zip(graphs, (a, b)):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for _, out, want, *_ in graphs:
+            _same(out, want)
+
+
+@pytest.mark.parametrize("name", PASSES)
+def test_on_other_streams_two_at_once(name):
+    ins, run = PASSES[name](0)
+    ins2, _ = PASSES[name](4)
+    want, want2 = run(*ins), run(*ins2)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for s, i in zip(streams, (ins, ins2)):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(run(*i))
+        torch.cuda.synchronize()
+        _same(got[0], want)
+        _same(got[1], want2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=["f32", "f16"])
+@pytest.mark.parametrize("name", PASSES)
+def test_nothing_depends_on_what_buffers_held(name, dtype):
+    """every entry point twice, outputs and workspaces filled with different poison before each: equal bits"""
+    from tests._poison import DoubleRun
+    ins, run = PASSES[name](0, dtype)
+    with DoubleRun(r"^icg_(attention|groupnorm|embedding)") as d:
+        with torch.autograd.set_multithreading_enabled(False):
+            run(*ins)
+    assert d.calls and not d.failures
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("spread,up", [(5.0, 1.0), (1.0, 2.0 ** -14), (1.0, 2.0 ** 9), (0.05, 1.0)], ids=["sharp", "small_gradient", "large_gradient", "flat"])
+@pytest.mark.parametrize("name", ["odd_lengths", "causal_square_packed"])
+def test_attention_values_far_from_one(name, spread, up, dtype):
+    from ic_gan_amd import ops
+    case = A.CASES[A.IDS.index(name)]
+    q, k, v, do, lens, start = A.make(case, dtype, "cuda", 3, spread)
+    do = (do.float() * up / spread).to(dtype)
+    o, lse = ops.attention(q, k, v, causal=case[8], scale=0.7, return_lse=True)
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    want = A.reference(case, dtype, q, k, v, do, scale=0.7)
+    for n, t in zip(("o", "lse", "dq", "dk", "dv"), (o, lse) + grads):
+        A.check(t, want[n], n)
+
+
+def test_attention_lengths_are_held_to_the_keys():
+    from ic_gan_amd import ops
+    q, k, v = (torch.randn(3, n, 2, 32, device="cuda") for n in (5, 40, 40))
+    a = ops.attention(q, k, v, k_lens=torch.tensor([99, -3, 40], device="cuda"))
+    b = ops.attention(q, k, v, k_lens=torch.tensor([40, 0, 40], dtype=torch.int32, device="cuda"))
+    assert torch.equal(a, b) and not a[1].any() and a[0].abs().sum() > 0
+    for start in (-(2 ** 31), 2 ** 31 - 1):
+        c = ops.attention(q, k, v, causal=True, q_start=torch.full((3,), start, dtype=torch.int32, device="cuda"))
+        assert torch.equal(c, ops.attention(q, k, v)) if start > 0 else not c.any()
+
+
+def test_attention_empty_and_partial_gradients():
+    from ic_gan_amd import ops
+    for B, Lq, Lk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
+        q, k, v = (torch.randn(B, n, 2, 16, device="cuda", requires_grad=True) for n in (Lq, Lk, Lk))
+        o = ops.attention(q, k, v)
+        assert o.shape == (B, Lq, 2, 16) and not o.any()
+        o.sum().backward()
+        assert all(t.grad.shape == t.shape and not t.grad.any() for t in (q, k, v))
+    q, k, v = (torch.randn(2, 33, 2, 16, device="cuda") for _ in range(3))
+    v.requires_grad_()
+    ops.attention(q, k, v).sum().backward()                 # (an expanded gradient)
+    assert torch.isfinite(v.grad).all() and abs(float(v.grad.sum()) - 2 * 33 * 2 * 16) < 1e-2 * 2 * 33 * 2 * 16
+    with pytest.raises(RuntimeError, match="differentiate twice|once_differentiable|trying to differentiate"):
+        o = ops.attention(q, k, v)
+        (g,) = torch.autograd.grad(o.square().sum(), v, create_graph=True)
+        g.sum().backward()
+
+
+def test_attention_far_addresses():
+    """positions 8 MB apart: the last keys lie 8 GB behind the first"""
+    from ic_gan_amd import ops
+    n, step = 1024, 4 << 20
+    buf = torch.empty(n * step, dtype=torch.bfloat16, device="cuda")
+    k, v = (buf.as_strided((1, n, 2, 64), (0, step, 64, 1), at) for at in (0, 128))
+    k.copy_(torch.randn(1, n, 2, 64, device="cuda")), v.copy_(torch.randn(1, n, 2, 64, device="cuda"))
+    for Lq in (1, 40):
+        q = torch.randn(1, Lq, 4, 64, device="cuda", dtype=torch.bfloat16)
+        assert torch.equal(ops.attention(q, k, v), ops.attention(q, k.contiguous(), v.contiguous()))
+    do = torch.randn(1, 40, 4, 64, device="cuda", dtype=torch.bfloat16)
+    got = []
+    for kk, vv in ((k, v), (k.contiguous(), v.contiguous())):
+        leaves = [t.detach().requires_grad_() for t in (q, kk, vv)]
+        got.append(torch.autograd.grad(ops.attention(*leaves), leaves, do))
+    _same(*got)
+
+
+def test_norm_far_addresses():
+    """5 GB of activations: the last sample's values equal those of the sample alone"""
+    from ic_gan_amd import ops
+    x = torch.empty(41, 64, 512, 1024, dtype=torch.bfloat16, device="cuda", memory_format=torch.channels_last)
+    x.normal_()
+    y = ops.group_norm_act(x, 8, act="silu")
+    last = ops.group_norm_act(x[-1:], 8, act="silu")
+    # (other chunks of the sums: equal statistics up to fp32 rounding, so outputs within one rounding step of bf16)
+    diff = (y[-1:].float() - last.float()).abs()
+    assert float((diff / (last.float().abs() + 1e-2)).max()) <= 2 ** -7
+
+
+def test_norm_takes_any_layout_and_type_of_gain():
+    from ic_gan_amd import ops
+    x = torch.randn(3, 24, 9, 7, device="cuda")
+    gain, bias = torch.randn(24, device="cuda").bfloat16(), torch.randn(24, device="cuda").bfloat16()
+    y = ops.group_norm_act(x, 4, gain, bias, act="relu")
+    z = ops.group_norm_act(x.contiguous(memory_format=torch.channels_last), 4, gain.float(), bias.float(), act="relu")
+    assert torch.equal(y, z)
+    only = ops.group_norm_act(x, 4, None, bias)
+    assert torch.equal(only, ops.group_norm_act(x, 4, torch.ones(24, device="cuda"), bias.float()))
+    e = ops.group_norm_act(x[:0], 4, gain, bias)
+    assert e.shape == (0, 24, 9, 7)
+
+
+def test_embedding_of_a_view_and_of_no_tokens():
+    from ic_gan_amd import ops
+    w = torch.randn(50, 40, device="cuda")[:, ::2].requires_grad_()
+    idx = torch.randint(0, 50, (6, 8), device="cuda").t()
+    out = ops.embedding(idx, w, scale=2.0)
+    assert torch.equal(out, torch.nn.functional.embedding(idx, w) * 2.0)
+    out.sum().backward()                                   # (an expanded gradient)
+    assert torch.equal(w.grad, 2.0 * torch.bincount(idx.flatten(), minlength=50).view(-1, 1).expand(50, 20).float())
+    w.grad = None
+    ops.embedding(idx[:0], w).sum().backward()
+    assert not w.grad.any()
+
+
+def test_large_label_table_takes_the_sorted_gradient():
+    """layers.SNEmbedding with a table too large for the one-hot product: the same gradient as the one-hot form's, in fp32 rounding"""
+    from ic_gan_amd import layers
+    torch.manual_seed(0)
+    m = layers.SNEmbedding(40000, 16).cuda().train()
+    y = torch.randint(0, 300, (2000,), device="cuda")
+    assert y.numel() * 40000 > 1 << 26
+    out = m(y)
+    d = torch.randn_like(out)
+    out.backward(d)
+    w = m.weight.detach().double()
+    u, v = m.u0.double(), None
+    v = torch.nn.functional.normalize(u @ w, dim=1)
+    sigma = (v @ w.t() @ u.t()).item()
+    raw = torch.zeros(40000, 16, dtype=torch.float64, device="cuda").index_add_(0, y, d.double())
+    want = (raw - (raw * w).sum() / sigma * (u.t() @ v)) / sigma
+    # u0 is the power iteration's next vector, u W / |u W| its partner within the iteration's own progress: 1e-2 of the correction term, which
+    # is far below the raw gradient's norm here
+    assert float((m.weight.grad.double() - want).norm()) <= 2e-2 * float(want.norm())
