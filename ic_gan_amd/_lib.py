@@ -150,9 +150,15 @@ def call(name: str, *args):
                 dev = a.get_device()
     if _raw_stream is not None and dev >= 0:
         st = _raw_stream(dev)
+        # a kernel goes to the current device, so that has to be the tensors' one (they may live on another)
+        if dev != torch._C._cuda_getDevice():
+            with torch.cuda.device(dev):
+                rc = fn(*conv, st)
+        else:
+            rc = fn(*conv, st)
     else:
         st = torch.cuda.current_stream().cuda_stream
-    rc = fn(*conv, st)
+        rc = fn(*conv, st)
     if rc != 0:
         l = lib()
         msg = l.icg_strerror(rc).decode()

@@ -8,7 +8,6 @@ is what the kernels address; `_cl` makes that true at module boundaries.
 """
 from __future__ import annotations
 
-import contextlib
 import os
 from dataclasses import dataclass, replace
 from typing import Optional
@@ -1323,26 +1322,30 @@ class AttnOutFn(Function):
 _DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _on_device(t: torch.Tensor):
-    """context: the operators launch on the device that holds their tensors, whichever is current"""
-    return torch.cuda.device(t.device) if t.is_cuda and t.get_device() != torch.cuda.current_device() else contextlib.nullcontext()
-
-
 def _rows_readable(t, width):
     """the tensor itself if the attention kernels can address its rows (whole 16-byte chunks at multiples of 16 bytes, positions at least a row
-    and less than 16 MB apart), else a copy with rows of `width` elements, zeros behind"""
-    size, e = t.element_size(), t.shape[-1]
-    if e == width and (t.stride(-1) == 1 or e == 1) and t.data_ptr() % 16 == 0:
-        sb, sl, sh = t.stride(0), t.stride(1), t.stride(2)
-        if e <= sl < (1 << 24) // size and not (sb * size) % 16 and not (sl * size) % 16 and not (sh * size) % 16:
-            return t
-    if e == width:
-        return t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
-    return torch.nn.functional.pad(t, (0, width - e)).contiguous()
+    and less than 16 MB apart), else a copy with rows of `width` elements, zeros behind; and its strides of batch, position and head"""
+    sb, sl, sh, se = t.stride()
+    e, per = t.shape[3], 16 // t.element_size()
+    if e == width and (se == 1 or e == 1) and e <= sl < (per << 20) and not (sb % per or sl % per or sh % per or t.data_ptr() % 16):
+        return t, (sb, sl, sh)
+    t = torch.nn.functional.pad(t, (0, width - e)).contiguous() if e != width else t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()[:3]
 
 
-def _strides3(t):
-    return t.stride(0), t.stride(1), t.stride(2)
+_PLANS = {}
+
+
+def _host_plan(*key):
+    """icg_*_applies / icg_*_workspace_bytes of the attention, group norm and embedding entry points by name and sizes.  They are functions of
+    the sizes alone, and small calls are bound by the host: remembered (per query function: tests replace it)."""
+    key = (L.query,) + key
+    n = _PLANS.get(key)
+    if n is None:
+        if len(_PLANS) >= 4096:
+            _PLANS.clear()
+        n = _PLANS[key] = L.query(*key[1:])
+    return n
 
 
 def _check_index_vector(name, t, B, like):
@@ -1352,7 +1355,29 @@ def _check_index_vector(name, t, B, like):
         raise ValueError("attention: %s must be an int32 or int64 tensor of shape [%d]" % (name, B))
     if t.device != like.device:
         raise ValueError("attention: %s is on %s, q on %s" % (name, t.device, like.device))
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _attention_forward(q, k, v, k_lens, q_start, scale, causal):
+    """-> (o, lse) and what the backward pass needs"""
+    B, Lq, H, d = q.shape
+    Lk, Hk, dv0 = k.shape[1], k.shape[2], v.shape[3]
+    dt, per = _DTYPE_CODES[q.dtype], 16 // q.element_size()
+    d, dv = -(-d // per) * per, -(-dv0 // per) * per
+    q, sq = _rows_readable(q, d)
+    k, sk = _rows_readable(k, d)
+    v, sv = _rows_readable(v, dv)
+    dev = q.device
+    o = torch.empty((B, Lq, H, dv), device=dev, dtype=q.dtype)
+    lse = torch.empty((B, H, Lq), device=dev, dtype=torch.float32)
+    if B * Lq * H == 0 or Lk == 0:
+        o.zero_()
+        lse.fill_(float("-inf"))
+    else:
+        nb = _host_plan("icg_attention_fwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, dt)
+        L.call("icg_attention_fwd", q, k, v, k_lens, q_start, o, lse, B, Lq, Lk, H, Hk, d, dv, *sq, *sk, *sv, scale, int(causal), dt,
+               _bytes(nb, dev) if nb else None, nb)
+    return (o if dv == dv0 else o[..., :dv0].contiguous()), lse, (q, k, v, o)
 
 
 class AttentionFn(Function):
@@ -1361,27 +1386,11 @@ class AttentionFn(Function):
 
     @staticmethod
     def forward(ctx, q, k, v, k_lens, q_start, scale, causal):
-        B, Lq, H, d = q.shape
-        Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
-        dt = _DTYPE_CODES[q.dtype]
-        ctx.widths = (d, dv)
-        per = 16 // q.element_size()
-        d, dv = -(-d // per) * per, -(-dv // per) * per
-        q, k, v = _rows_readable(q, d), _rows_readable(k, d), _rows_readable(v, dv)
-        o = torch.empty(B, Lq, H, dv, device=q.device, dtype=q.dtype)
-        lse = torch.empty(B, H, Lq, device=q.device, dtype=torch.float32)
-        if o.numel() == 0 or Lk == 0:
-            o.zero_()
-            lse.fill_(float("-inf"))
-        else:
-            with _on_device(q):
-                nb = L.query("icg_attention_fwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, dt)
-                L.call("icg_attention_fwd", q, k, v, k_lens, q_start, o, lse, B, Lq, Lk, H, Hk, d, dv, *_strides3(q), *_strides3(k), *_strides3(v),
-                       scale, int(causal), dt, _bytes(nb, q.device) if nb else None, nb)
-        ctx.scale, ctx.causal = scale, causal
-        ctx.save_for_backward(q, k, v, o, lse, k_lens, q_start)
+        ctx.widths, ctx.scale, ctx.causal = (q.shape[3], v.shape[3]), scale, causal
+        o, lse, kept = _attention_forward(q, k, v, k_lens, q_start, scale, causal)
+        ctx.save_for_backward(*kept, lse, k_lens, q_start)
         ctx.mark_non_differentiable(lse)
-        return (o if dv == ctx.widths[1] else o[..., :ctx.widths[1]].contiguous()), lse
+        return o, lse
 
     @staticmethod
     @once_differentiable
@@ -1389,16 +1398,15 @@ class AttentionFn(Function):
         q, k, v, o, lse, k_lens, q_start = ctx.saved_tensors
         B, Lq, H, d = q.shape
         Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
-        dt = _DTYPE_CODES[q.dtype]
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        dk, dv_ = torch.empty(k.shape, device=q.device, dtype=q.dtype), torch.empty(v.shape, device=q.device, dtype=q.dtype)
-        if o.numel() == 0 or Lk == 0:
-            return dq.zero_()[..., :ctx.widths[0]], dk.zero_()[..., :ctx.widths[0]], dv_.zero_()[..., :ctx.widths[1]], None, None, None, None
-        do = _rows_readable(do, dv)
-        with _on_device(q):
-            nb = L.query("icg_attention_bwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, int(ctx.causal), dt)
-            L.call("icg_attention_bwd", q, k, v, o, do, lse, k_lens, q_start, dq, dk, dv_, B, Lq, Lk, H, Hk, d, dv, *_strides3(q), *_strides3(k),
-                   *_strides3(v), *_strides3(do), ctx.scale, int(ctx.causal), dt, _bytes(nb, q.device), nb)
+        dt, dev = _DTYPE_CODES[q.dtype], q.device
+        dq, dk, dv_ = (torch.empty(t.shape, device=dev, dtype=q.dtype) for t in (q, k, v))
+        if B * Lq * H == 0 or Lk == 0:
+            dq.zero_(), dk.zero_(), dv_.zero_()
+        else:
+            do, sdo = _rows_readable(do, dv)
+            nb = _host_plan("icg_attention_bwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, int(ctx.causal), dt)
+            L.call("icg_attention_bwd", q, k, v, o, do, lse, k_lens, q_start, dq, dk, dv_, B, Lq, Lk, H, Hk, d, dv, *q.stride()[:3], *k.stride()[:3],
+                   *v.stride()[:3], *sdo, ctx.scale, int(ctx.causal), dt, _bytes(nb, dev), nb)
         if ctx.widths != (d, dv):
             dq, dk, dv_ = dq[..., :ctx.widths[0]], dk[..., :ctx.widths[0]], dv_[..., :ctx.widths[1]]
         return dq, dk, dv_, None, None, None, None
@@ -1419,13 +1427,14 @@ def attention(q, k, v, *, scale=None, causal=False, k_lens=None, q_start=None, r
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not isinstance(t, torch.Tensor) or t.dim() != 4:
             raise ValueError("attention: %s must be a 4-D tensor [batch, position, head, element]" % name)
-        if t.dtype != q.dtype or t.device != q.device:
-            raise ValueError("attention: q, k and v must have one type and device (q %s on %s, %s %s on %s)" % (q.dtype, q.device, name, t.dtype, t.device))
-    if q.dtype not in _DTYPE_CODES:
-        raise ValueError("attention: fp32, fp16 or bf16, not %s" % q.dtype)
-    B, Lq, H, d = q.shape
-    Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
-    if k.shape[0] != B or v.shape[0] != B or v.shape[1] != Lk or v.shape[2] != Hk or k.shape[3] != d:
+    dtype, dev = q.dtype, q.device
+    if k.dtype != dtype or v.dtype != dtype or k.device != dev or v.device != dev:
+        raise ValueError("attention: q, k and v must have one type and device (q %s on %s, k %s on %s, v %s on %s)" % (
+            dtype, dev, k.dtype, k.device, v.dtype, v.device))
+    if dtype not in _DTYPE_CODES:
+        raise ValueError("attention: fp32, fp16 or bf16, not %s" % dtype)
+    (B, Lq, H, d), (Bk, Lk, Hk, dk), (Bv, Lv, Hv, dv) = q.shape, k.shape, v.shape
+    if Bk != B or Bv != B or Lv != Lk or Hv != Hk or dk != d:
         raise ValueError("attention: shapes do not fit: q %s, k %s, v %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     if Hk == 0 or H % Hk != 0:
         raise ValueError("attention: %d query heads over %d key heads" % (H, Hk))
@@ -1435,9 +1444,12 @@ def attention(q, k, v, *, scale=None, causal=False, k_lens=None, q_start=None, r
     if not (0.0 < scale < float("inf")):
         raise ValueError("attention: scale must be positive and finite, not %r" % scale)
     k_lens, q_start = _check_index_vector("k_lens", k_lens, B, q), _check_index_vector("q_start", q_start, B, q)
-    if B * Lq * Lk and not L.query("icg_attention_applies", B, Lq, Lk, H, Hk, -(-d // 8) * 8, -(-dv // 8) * 8, _DTYPE_CODES[q.dtype]):
+    if B * Lq * Lk and not _host_plan("icg_attention_applies", B, Lq, Lk, H, Hk, -(-d // 8) * 8, -(-dv // 8) * 8, _DTYPE_CODES[dtype]):
         raise ValueError("attention: not served: B %d, Lq %d, Lk %d, H %d, d %d, dv %d (d, dv <= 128, or d <= 64 and dv <= 256)" % (B, Lq, Lk, H, d, dv))
     _require_gpu(q)
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        o, lse, _ = _attention_forward(q, k, v, k_lens, q_start, scale, bool(causal))
+        return (o, lse) if return_lse else o
     o, lse = AttentionFn.apply(q, k, v, k_lens, q_start, scale, bool(causal))
     return (o, lse) if return_lse else o
 
@@ -1470,10 +1482,9 @@ class GroupNormActFn(Function):
         mean, rstd = _f32(B * groups, x.device), _f32(B * groups, x.device)
         ctx.meta = (groups, per_sample, gain_offset, eps, act, dt)
         if x.numel():
-            with _on_device(x):
-                nb = L.query("icg_groupnorm_fwd_workspace_bytes", B, H * W, C, groups, dt)
-                L.call("icg_groupnorm_act_fwd", x, gain, bias, y, mean, rstd, B, H * W, C, groups, per_sample, gain_offset, eps, act, dt,
-                       _bytes(nb, x.device) if nb else None, nb)
+            nb = _host_plan("icg_groupnorm_fwd_workspace_bytes", B, H * W, C, groups, dt)
+            L.call("icg_groupnorm_act_fwd", x, gain, bias, y, mean, rstd, B, H * W, C, groups, per_sample, gain_offset, eps, act, dt,
+                   _bytes(nb, x.device) if nb else None, nb)
         ctx.save_for_backward(x, gain, bias, mean, rstd)
         return y
 
@@ -1490,10 +1501,9 @@ class GroupNormActFn(Function):
             shape = (B, C) if per_sample else (C,)
             dgain, dbias = (torch.empty(shape, device=x.device, dtype=torch.float32) for _ in range(2))
         if x.numel():
-            with _on_device(x):
-                nb = L.query("icg_groupnorm_bwd_workspace_bytes", B, H * W, C, groups, dt)
-                L.call("icg_groupnorm_act_bwd", x, dy, gain, bias, mean, rstd, dx, dgain, dbias, B, H * W, C, groups, per_sample, gain_offset, eps,
-                       act, dt, _bytes(nb, x.device), nb)
+            nb = _host_plan("icg_groupnorm_bwd_workspace_bytes", B, H * W, C, groups, dt)
+            L.call("icg_groupnorm_act_bwd", x, dy, gain, bias, mean, rstd, dx, dgain, dbias, B, H * W, C, groups, per_sample, gain_offset, eps,
+                   act, dt, _bytes(nb, x.device), nb)
         elif dgain is not None:
             dgain.zero_(), dbias.zero_()
         return dx, (dgain if gain is not None else None), (dbias if bias is not None else None), None, None, None, None
@@ -1535,16 +1545,15 @@ def group_norm_act(x, groups, gain=None, bias=None, *, eps=1e-5, act="none", gai
 # ----------------------------------------------------------------------------------------------
 def embedding_backward(idx, dout, V, scale=1.0, padding_idx=None):
     """[V, D]: scale times the sum of dout's rows over the positions of each token, in the order of the positions (icg_embedding_bwd)."""
-    D = dout.shape[-1]
-    flat, d2 = idx.reshape(-1).contiguous(), dout.reshape(-1, D).contiguous()
-    dw = torch.empty(V, D, device=dout.device, dtype=dout.dtype)
-    if flat.numel() == 0 or dw.numel() == 0:
+    D, flat = dout.shape[-1], idx.contiguous()
+    n, d2 = flat.numel(), dout.contiguous()
+    dw = torch.empty((V, D), device=dout.device, dtype=dout.dtype)
+    if n == 0 or dw.numel() == 0:
         return dw.zero_()
     dt = _DTYPE_CODES[dout.dtype]
-    with _on_device(dout):
-        nb = L.query("icg_embedding_bwd_workspace_bytes", flat.numel(), V, D, dt)
-        L.call("icg_embedding_bwd", flat, d2, dw, flat.numel(), V, D, scale, -1 if padding_idx is None else padding_idx, int(flat.dtype == torch.int64),
-               dt, _bytes(nb, dout.device) if nb else None, nb)
+    nb = _host_plan("icg_embedding_bwd_workspace_bytes", n, V, D, dt)
+    L.call("icg_embedding_bwd", flat, d2, dw, n, V, D, scale, -1 if padding_idx is None else padding_idx, int(flat.dtype == torch.int64),
+           dt, _bytes(nb, dout.device) if nb else None, nb)
     return dw
 
 
@@ -1555,8 +1564,7 @@ class EmbeddingFn(Function):
         V, D = w.shape
         out = torch.empty(*idx.shape, D, device=w.device, dtype=w.dtype)
         if out.numel():
-            with _on_device(w):
-                L.call("icg_embedding_fwd", flat, w, out, flat.numel(), V, D, scale, int(flat.dtype == torch.int64), _DTYPE_CODES[w.dtype])
+            L.call("icg_embedding_fwd", flat, w, out, flat.numel(), V, D, scale, int(flat.dtype == torch.int64), _DTYPE_CODES[w.dtype])
         ctx.meta = (V, scale, padding_idx)
         ctx.save_for_backward(flat)
         return out
