@@ -248,9 +248,9 @@ __device__ __forceinline__ int64_t at_work_item(int64_t n) {
 int at_fwd_f32(const AttnP&, bool tokens, hipStream_t);
 int at_fwd_f16(const AttnP&, bool tokens, hipStream_t);
 int at_fwd_bf16(const AttnP&, bool tokens, hipStream_t);
-int at_bwd_f32(const AttnP&, float* stat, hipStream_t);
-int at_bwd_f16(const AttnP&, float* stat, hipStream_t);
-int at_bwd_bf16(const AttnP&, float* stat, hipStream_t);
+int at_bwd_f32(const AttnP& dq, const AttnP& dkv, float* stat, hipStream_t);
+int at_bwd_f16(const AttnP& dq, const AttnP& dkv, float* stat, hipStream_t);
+int at_bwd_bf16(const AttnP& dq, const AttnP& dkv, float* stat, hipStream_t);
 // (DP, DVP): the head dimensions a kernel is built for.  A head takes the first pair that covers it: equal dimensions, and values up to four
 // times as wide as the keys, as the image models' blocks have them.
 #define AT_FOR_HEAD(d, dv, RUN)                               \

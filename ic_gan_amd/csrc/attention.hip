@@ -8,25 +8,35 @@ constexpr int kTokenRows = 32;     // rows of the kernel for few queries
 // Few queries: a 128-row tile would be mostly padding, and the heads that share a key head would each read it again.
 bool at_tokens(int Lq, int G) { return Lq <= 16 || (int64_t)Lq * G <= kTokenRows; }
 
-// How the keys are split over workgroups: with few queries two workgroups for each of the 256 compute units (what is read is all that counts,
-// and it takes two to keep the memory busy), with many one for each; no split shorter than 256 keys (below that the join costs more than it
-// saves).
-void at_plan(AttnP& p) {
-  const bool tok = at_tokens(p.Lq, p.G);
-  p.tiles = (int)(tok ? icg_cdiv((int64_t)p.Lq * p.G, kTokenRows) : icg_cdiv(p.Lq, 128));
-  const int64_t items = (int64_t)p.B * (tok ? p.H / p.G : p.H) * p.tiles, want = tok ? 512 : 256, unit = 256;
-  const int64_t most = icg_cdiv(p.Lk, unit);
+// The keys in splits for `want` workgroups, no split shorter than 256 keys (below that the join costs more than it saves); 3/4 of the wanted
+// number is enough
+void at_split_keys(AttnP& p, int64_t items, int64_t want) {
+  const int64_t unit = 256, most = icg_cdiv(p.Lk, unit);
   int64_t n = 4 * items >= 3 * want ? 1 : icg_cdiv(want, items);
   n = n < most ? n : most;
   n = n > 1 ? n : 1;
   p.keys_per_split = (int)(icg_cdiv(icg_cdiv(p.Lk, n), unit) * unit);
-  p.nsplit = (int)(p.Lk > 0 ? icg_cdiv(p.Lk, p.keys_per_split) : 1);
+  p.nsplit = (int)icg_cdiv(p.Lk, p.keys_per_split);
   p.work = items * p.nsplit;
+}
+
+// Forward: with few queries two workgroups for each of the 256 compute units (what is read is all that counts, and it takes two to keep the
+// memory busy), with many one for each.
+void at_plan(AttnP& p) {
+  const bool tok = at_tokens(p.Lq, p.G);
+  p.tiles = (int)(tok ? icg_cdiv((int64_t)p.Lq * p.G, kTokenRows) : icg_cdiv(p.Lq, 128));
+  at_split_keys(p, (int64_t)p.B * (tok ? p.H / p.G : p.H) * p.tiles, tok ? 512 : 256);
+}
+
+// dq
+void at_plan_dq(AttnP& p) {
+  p.tiles = (int)icg_cdiv(p.Lq, 128);
+  at_split_keys(p, (int64_t)p.B * p.H * p.tiles, 256);
 }
 
 // How the queries of a key tile are split in the key gradient: a workgroup for each compute unit, twice as many where a causal triangle makes
 // them uneven (the long ones start first and the short ones fill up behind them); at least 4 query tiles each
-void at_plan_bwd(AttnP& p) {
+void at_plan_dkv(AttnP& p) {
   p.tiles = (int)icg_cdiv(p.Lk, 128);
   const int64_t items = (int64_t)p.B * (p.H / p.G) * p.tiles, steps = (int64_t)p.G * icg_cdiv(p.Lq, 64), want = p.causal ? 512 : 256;
   int64_t n = 4 * items >= 3 * want ? 1 : icg_cdiv(want, items);
@@ -36,8 +46,10 @@ void at_plan_bwd(AttnP& p) {
   p.work = items * p.nsplit;
 }
 size_t at_stat_bytes(const AttnP& p) { return ((size_t)3 * p.B * p.H * p.Lq * 4 + 15) / 16 * 16; }
-size_t at_bwd_bytes(const AttnP& p) {
-  return at_stat_bytes(p) + (p.nsplit > 1 ? (size_t)p.nsplit * p.B * p.Lk * (p.H / p.G) * (p.d + p.dv) * 4 : 0);
+size_t at_bwd_bytes(const AttnP& dq, const AttnP& dkv) {
+  const size_t a = dq.nsplit > 1 ? (size_t)dq.nsplit * dq.B * dq.H * dq.Lq * dq.d * 4 : 0;
+  const size_t b = dkv.nsplit > 1 ? (size_t)dkv.nsplit * dkv.B * dkv.Lk * (dkv.H / dkv.G) * (dkv.d + dkv.dv) * 4 : 0;
+  return at_stat_bytes(dq) + (a > b ? a : b);
 }
 
 size_t at_part_bytes(const AttnP& p) {
@@ -76,8 +88,10 @@ extern "C" size_t icg_attention_bwd_workspace_bytes(int B, int Lq, int Lk, int H
   if (!at_shape_ok(B, Lq, Lk, H, Hk, d, dv, dtype)) return 0;
   AttnP p = {};
   p.B = B, p.Lq = Lq, p.Lk = Lk, p.H = H, p.G = H / Hk, p.d = d, p.dv = dv, p.causal = causal != 0;
-  at_plan_bwd(p);
-  return at_bwd_bytes(p);
+  AttnP pk = p;
+  at_plan_dq(p);
+  at_plan_dkv(pk);
+  return at_bwd_bytes(p, pk);
 }
 
 extern "C" int icg_attention_fwd(const void* q, const void* k, const void* v, const int* k_lens, const int* q_start, void* o, float* lse, int B,
@@ -125,10 +139,12 @@ extern "C" int icg_attention_bwd(const void* q, const void* k, const void* v, co
   p.scale = scale, p.causal = causal != 0;
   ICG_REQUIRE(at_row_ok(q, q_sb, q_sl, q_sh, d, size) && at_row_ok(k, k_sb, k_sl, k_sh, d, size) && at_row_ok(v, v_sb, v_sl, v_sh, dv, size));
   ICG_REQUIRE(at_row_ok(dout, do_sb, do_sl, do_sh, dv, size));
-  at_plan_bwd(p);
-  ICG_REQUIRE(p.work < 0x7fffffffL);
   float* stat = (float*)workspace;
   p.part = (float*)((char*)workspace + at_stat_bytes(p));
+  AttnP pk = p;
+  at_plan_dq(p);
+  at_plan_dkv(pk);
+  ICG_REQUIRE(p.work < 0x7fffffffL && pk.work < 0x7fffffffL);
   hipStream_t st = (hipStream_t)stream;
-  return dtype == 0 ? at_bwd_f32(p, stat, st) : dtype == 1 ? at_bwd_f16(p, stat, st) : at_bwd_bf16(p, stat, st);
+  return dtype == 0 ? at_bwd_f32(p, pk, stat, st) : dtype == 1 ? at_bwd_f16(p, pk, stat, st) : at_bwd_bf16(p, pk, stat, st);
 }

@@ -4,29 +4,28 @@
 #pragma once
 #include "attention.h"
 
-// D_i = do_i . o_i, |do_i| and the exponent's offset, a row per 32 lanes; rows in memory order
+// D_i = do_i . o_i, |do_i| and the exponent's offset; `lanes` lanes (the power of two that covers a row's 16-byte chunks) to a row, rows in
+// memory order
 template <typename T>
-__global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, float* stat) {
-  const int64_t rows = (int64_t)p.B * p.H * p.Lq, i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int l = threadIdx.x & 31;
+__global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, float* stat, int lanes) {
+  const int64_t rows = (int64_t)p.B * p.H * p.Lq, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int l = threadIdx.x & (lanes - 1);
   if (i >= rows) return;
   const int64_t bq = i / p.H;
   const int hq = (int)(i - bq * p.H);
   const int64_t b = bq / p.Lq, qi = bq - b * p.Lq;
-  const T* o = reinterpret_cast<const T*>(p.o) + i * p.dv;
-  const T* g = reinterpret_cast<const T*>(p.dout) + b * p.do_sb + qi * p.do_sl + hq * p.do_sh;
   constexpr int PER = 16 / (int)sizeof(T);
   float dot = 0.f, sq = 0.f;
-  for (int c = l; c * PER < p.dv; c += 32) {
-    const at_u4 a = *reinterpret_cast<const at_u4*>(o + c * PER), e = *reinterpret_cast<const at_u4*>(g + c * PER);
+  if (l * PER < p.dv) {
+    const at_u4 a = *reinterpret_cast<const at_u4*>(reinterpret_cast<const T*>(p.o) + i * p.dv + l * PER);
+    const at_u4 e = *reinterpret_cast<const at_u4*>(reinterpret_cast<const T*>(p.dout) + b * p.do_sb + qi * p.do_sl + hq * p.do_sh + l * PER);
     T x[PER], y[PER];
     __builtin_memcpy(x, &a, 16);
     __builtin_memcpy(y, &e, 16);
 #pragma unroll
     for (int j = 0; j < PER; ++j) dot = __builtin_fmaf((float)x[j], (float)y[j], dot), sq = __builtin_fmaf((float)y[j], (float)y[j], sq);
   }
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor(dot, s, 64), sq += __shfl_xor(sq, s, 64);
+  for (int s = lanes >> 1; s > 0; s >>= 1) dot += __shfl_xor(dot, s, 64), sq += __shfl_xor(sq, s, 64);
   if (l == 0) {
     const int64_t row = (b * p.H + hq) * p.Lq + qi;
     const float lse = p.lse[row];
@@ -48,7 +47,7 @@ __device__ __forceinline__ float at_ds(float pr, float dp, float s, float delta_
   return x;
 }
 
-// dq: a workgroup owns 128 queries of one head (a wave 32, as columns) and streams the keys
+// dq: a workgroup owns 128 queries of one head (a wave 32, as columns) and streams the keys, or its split of them
 template <typename T, int DP, int DVP> constexpr int at_dq_waves() { return (DP + DVP) * (int)sizeof(T) / 8 + DP / 2 <= 144 ? 2 : 1; }
 template <typename T, int DP, int DVP>
 __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attention_dq_kernel(AttnP p) {
@@ -58,7 +57,9 @@ __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attentio
   __shared__ __attribute__((aligned(64))) char lds[2 * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 31, h = lane >> 5;
-  const int64_t item = at_work_item(p.work);
+  int64_t item = at_work_item(p.work);
+  const int split = (int)(item % p.nsplit);
+  item /= p.nsplit;
   int tile = (int)(item % p.tiles);
   const int64_t bh = item / p.tiles;
   const int b = (int)(bh / p.H), hq = (int)(bh - (int64_t)b * p.H), hk = hq / p.G;
@@ -67,7 +68,9 @@ __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attentio
   const bool valid = qi < p.Lq;
   const int keys = at_keys(p, b), start = at_start(p, b);
   const int last = !valid ? -1 : (p.causal ? min(keys - 1, start + qi) : keys - 1);
-  const int kend = p.causal ? min(keys, start + min(p.Lq - 1, 128 * tile + 127) + 1) : keys;
+  int kend = p.causal ? min(keys, start + min(p.Lq - 1, 128 * tile + 127) + 1) : keys;
+  const int k0 = split * p.keys_per_split;
+  if (p.nsplit > 1) kend = min(kend, k0 + p.keys_per_split);
 
   frag qf[DP / X::KSTEP], gf[DVP / X::KSTEP];
   at_own<T, DP>(qf, reinterpret_cast<const T*>(p.q) + b * p.q_sb + qi * p.q_sl + hq * p.q_sh, valid, p.d, h);
@@ -98,13 +101,13 @@ __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attentio
     vs.put(lds + cur * SLOT + KBYTES, tid);
   };
   int cur = 0;
-  if (kend > 0) {
-    fetch(0);
+  if (k0 < kend) {
+    fetch(k0);
     put(0);
-    if (KT < kend) fetch(KT);
+    if (k0 + KT < kend) fetch(k0 + KT);
     __syncthreads();
   }
-  for (int j0 = 0; j0 < kend; j0 += KT) {
+  for (int j0 = k0; j0 < kend; j0 += KT) {
     const char* kt = lds + cur * SLOT;
     const char* vt = kt + KBYTES;
 #pragma unroll
@@ -140,6 +143,15 @@ __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attentio
   }
   if (!valid) return;
   const float f = p.scale * (1.f / (1 << X::P_SHIFT)) / s1;
+  if (p.nsplit > 1) {
+    float* out = p.part + (split * rows + row) * p.d;
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        at_store4<float>(out, 32 * c + 8 * g + 4 * h, p.d, acc[c][4 * g] * f, acc[c][4 * g + 1] * f, acc[c][4 * g + 2] * f, acc[c][4 * g + 3] * f);
+    return;
+  }
   T* out = reinterpret_cast<T*>(p.dq) + (((int64_t)b * p.Lq + qi) * p.H + hq) * p.d;
 #pragma unroll
   for (int c = 0; c < DP / 32; ++c)
@@ -328,6 +340,20 @@ __global__ __launch_bounds__(256, (at_dkv_shape<T, DP, DVP>::WAVES)) void icg_at
       at_store4<T>(dv_out, 32 * c + 8 * g + 4 * h, p.dv, dv[c][4 * g] * fv, dv[c][4 * g + 1] * fv, dv[c][4 * g + 2] * fv, dv[c][4 * g + 3] * fv);
 }
 
+// sums the splits of dq in order: a thread takes 4 elements of a row
+template <typename T>
+__global__ __launch_bounds__(256) void icg_attention_join_dq_kernel(AttnP p) {
+  const int64_t rows = (int64_t)p.B * p.H * p.Lq;
+  const int quads = p.d / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / quads;
+  if (row >= rows) return;
+  const int c = (int)(i - row * quads) * 4;
+  at_f4 x = *reinterpret_cast<const at_f4*>(p.part + row * p.d + c);
+  for (int s = 1; s < p.nsplit; ++s) x += *reinterpret_cast<const at_f4*>(p.part + (s * rows + row) * p.d + c);
+  const int64_t bh = row / p.Lq, qi = row - bh * p.Lq, b = bh / p.H, hq = bh - b * p.H;
+  at_store4<T>(reinterpret_cast<T*>(p.dq) + ((b * p.Lq + qi) * p.H + hq) * p.d, c, p.d, x[0], x[1], x[2], x[3]);
+}
+
 // sums the splits of dk and dv in order: a thread takes 4 elements of a key's row [d + dv]
 template <typename T>
 __global__ __launch_bounds__(256) void icg_attention_join_dkv_kernel(AttnP p) {
@@ -342,25 +368,29 @@ __global__ __launch_bounds__(256) void icg_attention_join_dkv_kernel(AttnP p) {
   else at_store4<T>(reinterpret_cast<T*>(p.dv_out) + row * p.dv, c - p.d, p.dv, x[0], x[1], x[2], x[3]);
 }
 
+// p: planned for dq, pk: for dk and dv; the two take turns with the room for partial sums
 template <typename T>
-int at_bwd(const AttnP& in, float* stat, hipStream_t st) {
-  AttnP p = in;
-  p.stat = stat;
-  hipLaunchKernelGGL((icg_attention_rowstat_kernel<T>), dim3((unsigned)icg_cdiv((int64_t)p.B * p.H * p.Lq, 8)), dim3(256), 0, st, p, stat);
+int at_bwd(AttnP p, AttnP pk, float* stat, hipStream_t st) {
+  p.stat = pk.stat = stat;
+  int lanes = 1;
+  while (lanes * 16 < p.dv * (int)sizeof(T)) lanes <<= 1;        // (at most 64: rows of up to 256 fp32)
+  hipLaunchKernelGGL((icg_attention_rowstat_kernel<T>), dim3((unsigned)icg_cdiv((int64_t)p.B * p.H * p.Lq * lanes, 256)), dim3(256), 0, st, p, stat, lanes);
   if (const int e = icg_check_launch()) return e;
-  const AttnP pk = p;                                    // (planned by the caller: key tiles and splits)
-  p.tiles = (int)icg_cdiv(p.Lq, 128);
-  p.work = (int64_t)p.B * p.H * p.tiles;
-#define AT_RUN(DP, DVP)                                                                                                 \
-  do {                                                                                                                  \
-    hipLaunchKernelGGL((icg_attention_dkv_kernel<T, DP, DVP>), dim3((unsigned)pk.work), dim3(256), 0, st, pk);          \
-    if (const int e = icg_check_launch()) return e;                                                                     \
-    if (pk.nsplit > 1) {                                                                                                \
-      const int64_t quads = (int64_t)p.B * p.Lk * (p.H / p.G) * ((p.d + p.dv) / 4);                                     \
+#define AT_RUN(DP, DVP)                                                                                                  \
+  do {                                                                                                                   \
+    hipLaunchKernelGGL((icg_attention_dkv_kernel<T, DP, DVP>), dim3((unsigned)pk.work), dim3(256), 0, st, pk);           \
+    if (const int e = icg_check_launch()) return e;                                                                      \
+    if (pk.nsplit > 1) {                                                                                                 \
+      const int64_t quads = (int64_t)p.B * p.Lk * (p.H / p.G) * ((p.d + p.dv) / 4);                                      \
       hipLaunchKernelGGL((icg_attention_join_dkv_kernel<T>), dim3((unsigned)icg_cdiv(quads, 256)), dim3(256), 0, st, pk); \
-      if (const int e = icg_check_launch()) return e;                                                                   \
-    }                                                                                                                   \
-    hipLaunchKernelGGL((icg_attention_dq_kernel<T, DP, DVP>), dim3((unsigned)p.work), dim3(256), 0, st, p);             \
+      if (const int e = icg_check_launch()) return e;                                                                    \
+    }                                                                                                                    \
+    hipLaunchKernelGGL((icg_attention_dq_kernel<T, DP, DVP>), dim3((unsigned)p.work), dim3(256), 0, st, p);              \
+    if (p.nsplit > 1) {                                                                                                  \
+      if (const int e = icg_check_launch()) return e;                                                                    \
+      const int64_t quads = (int64_t)p.B * p.H * p.Lq * (p.d / 4);                                                       \
+      hipLaunchKernelGGL((icg_attention_join_dq_kernel<T>), dim3((unsigned)icg_cdiv(quads, 256)), dim3(256), 0, st, p);  \
+    }                                                                                                                    \
   } while (0)
   AT_FOR_HEAD(p.d, p.dv, AT_RUN)
 #undef AT_RUN

@@ -3,4 +3,4 @@
 #include "attention_bwd.h"
 
 int at_fwd_f16(const AttnP& p, bool tokens, hipStream_t st) { return at_fwd<_Float16>(p, tokens, st); }
-int at_bwd_f16(const AttnP& p, float* stat, hipStream_t st) { return at_bwd<_Float16>(p, stat, st); }
+int at_bwd_f16(const AttnP& dq, const AttnP& dkv, float* stat, hipStream_t st) { return at_bwd<_Float16>(dq, dkv, stat, st); }

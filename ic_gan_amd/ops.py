@@ -1333,6 +1333,15 @@ def _rows_readable(t, width):
     return t, t.stride()[:3]
 
 
+def _first_order(backward):
+    """once_differentiable, without its detour where no second derivative can be asked for (a small call's backward pass is bound by the host)"""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 _PLANS = {}
 
 
@@ -1393,7 +1402,7 @@ class AttentionFn(Function):
         return o, lse
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, do, dlse=None):
         q, k, v, o, lse, k_lens, q_start = ctx.saved_tensors
         B, Lq, H, d = q.shape
@@ -1489,7 +1498,7 @@ class GroupNormActFn(Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, gain, bias, mean, rstd = ctx.saved_tensors
         groups, per_sample, gain_offset, eps, act, dt = ctx.meta
@@ -1498,8 +1507,8 @@ class GroupNormActFn(Function):
         dx = torch.empty_like(x)
         dgain = dbias = None
         if gain is not None or bias is not None:
-            shape = (B, C) if per_sample else (C,)
-            dgain, dbias = (torch.empty(shape, device=x.device, dtype=torch.float32) for _ in range(2))
+            affine = gain if gain is not None else bias
+            dgain, dbias = torch.empty_like(affine), torch.empty_like(affine)
         if x.numel():
             nb = _host_plan("icg_groupnorm_bwd_workspace_bytes", B, H * W, C, groups, dt)
             L.call("icg_groupnorm_act_bwd", x, dy, gain, bias, mean, rstd, dx, dgain, dbias, B, H * W, C, groups, per_sample, gain_offset, eps,
@@ -1570,7 +1579,7 @@ class EmbeddingFn(Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         (flat,) = ctx.saved_tensors
         V, scale, padding_idx = ctx.meta
