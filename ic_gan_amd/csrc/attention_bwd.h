@@ -43,7 +43,7 @@ __device__ __forceinline__ float at_to_one(float norm) {
 template <typename T>
 __device__ __forceinline__ float at_ds(float pr, float dp, float s, float delta_s) {
   const float x = pr * __builtin_fmaf(dp, s, -delta_s);
-  if constexpr (at_type<T>::SCALED) return __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f);
+  if constexpr (at_type<T>::SCALED) return __builtin_isfinite(x) ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x;      // (inf and NaN stay visible)
   return x;
 }
 

@@ -1364,7 +1364,9 @@ def _check_index_vector(name, t, B, like):
         raise ValueError("attention: %s must be an int32 or int64 tensor of shape [%d]" % (name, B))
     if t.device != like.device:
         raise ValueError("attention: %s is on %s, q on %s" % (name, t.device, like.device))
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+    return t.contiguous()
 
 
 def _attention_forward(q, k, v, k_lens, q_start, scale, causal):
@@ -1399,11 +1401,14 @@ class AttentionFn(Function):
         o, lse, kept = _attention_forward(q, k, v, k_lens, q_start, scale, causal)
         ctx.save_for_backward(*kept, lse, k_lens, q_start)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)               # (no tensor of zeros for lse)
         return o, lse
 
     @staticmethod
     @_first_order
     def backward(ctx, do, dlse=None):
+        if do is None:
+            return (None,) * 7
         q, k, v, o, lse, k_lens, q_start = ctx.saved_tensors
         B, Lq, H, d = q.shape
         Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]

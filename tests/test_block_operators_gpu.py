@@ -165,6 +165,8 @@ def test_attention_lengths_are_held_to_the_keys():
     a = ops.attention(q, k, v, k_lens=torch.tensor([99, -3, 40], device="cuda"))
     b = ops.attention(q, k, v, k_lens=torch.tensor([40, 0, 40], dtype=torch.int32, device="cuda"))
     assert torch.equal(a, b) and not a[1].any() and a[0].abs().sum() > 0
+    d = ops.attention(q, k, v, k_lens=torch.tensor([2 ** 40, -(2 ** 40), 2 ** 33 + 3], device="cuda"))      # (held to, not wrapped)
+    assert torch.equal(d, b)
     for start in (-(2 ** 31), 2 ** 31 - 1):
         c = ops.attention(q, k, v, causal=True, q_start=torch.full((3,), start, dtype=torch.int32, device="cuda"))
         assert torch.equal(c, ops.attention(q, k, v)) if start > 0 else not c.any()
@@ -186,6 +188,28 @@ def test_attention_empty_and_partial_gradients():
         o = ops.attention(q, k, v)
         (g,) = torch.autograd.grad(o.square().sum(), v, create_graph=True)
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_attention_non_finite_gradients_stay_visible(dtype, bad):
+    """an overflown gradient (loss scaling looks for it) reaches every gradient that it is part of, and no other sequence"""
+    from ic_gan_amd import ops
+    q, k, v = (torch.randn(2, 40, 2, 32, device="cuda", dtype=dtype, requires_grad=True) for _ in range(3))
+    do = torch.randn(2, 40, 2, 32, device="cuda", dtype=dtype)
+    do[0, 7, 1, 5] = bad
+    dq, dk, dv = torch.autograd.grad(ops.attention(q, k, v), (q, k, v), do)
+    assert not torch.isfinite(dq[0, 7, 1]).any() and torch.isfinite(dq[1]).all() and torch.isfinite(dq[0, :, 0]).all()
+    assert not torch.isfinite(dk[0, :, 1]).any() and torch.isfinite(dk[1]).all()
+    assert not torch.isfinite(dv[0, :, 1, 5]).any() and torch.isfinite(dv[1]).all()
+
+
+def test_attention_log_sums_alone():
+    from ic_gan_amd import ops
+    q, k, v = (torch.randn(2, 9, 2, 16, device="cuda", requires_grad=True) for _ in range(3))
+    o, lse = ops.attention(q, k, v, return_lse=True)
+    (o.sum() + lse.detach().sum()).backward()
+    assert all(torch.isfinite(t.grad).all() for t in (q, k, v))
 
 
 def test_attention_far_addresses():
