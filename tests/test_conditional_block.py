@@ -123,3 +123,23 @@ def test_norm_style_is_checked():
     assert layers.norm_groups("bn") is None and layers.norm_groups("gn") == 16 and layers.norm_groups("gn_32") == 32
     with pytest.raises(NotImplementedError):
         layers.Embedding(4, 4, sparse=True)
+
+
+@pytest.mark.gpu
+def test_captured_generator_with_the_operators():
+    """sampling from a captured graph: bit-equal to the eager generator on every replay, with other work between"""
+    import ic_gan_amd.BigGAN as M
+    from ic_gan_amd import inference
+    flags = dict(norm_style="gn_%d" % GROUPS, attn_recompute=True, sorted_embedding=True, skip_init=True, embedded_optimizers=False)
+    G = M.Generator(**{**CFG, **flags})
+    G.load_state_dict(synth.synth_state(synth.spec_of(G.state_dict()), 11))
+    G = G.cuda().eval()
+    graphed = inference.GraphedGenerator(G, 4, class_cond=True, instance_cond=True, device="cuda:0")
+    for seed in range(3):
+        g = torch.Generator().manual_seed(seed)
+        z, feats = torch.randn(4, G.dim_z, generator=g).cuda(), F.normalize(torch.randn(4, 2048, generator=g), dim=1).cuda()
+        label = torch.randint(0, 10, (4,), generator=g).cuda()
+        with torch.no_grad():
+            want = G(z, label, feats).clone()
+        got = graphed(z, label, feats)
+        assert torch.equal(got, want)
