@@ -41,7 +41,7 @@ struct AttnP {
   float scale;
   int causal;                               // (every row of q, k, v, o, do starts at a multiple of 16 bytes and holds whole 16-byte chunks)
   // forward
-  void* o;
+  void *o, *o_low;                          // o_low: what the rounding of o took away, NULL if nobody asks
   float* lse;
   float* part;                              // split over the keys: [split][B][H][Lq] rows of dv sums, then their (maximum, sum) pairs
   int nsplit, keys_per_split;
@@ -232,6 +232,14 @@ __device__ __forceinline__ void at_store4(T* row, int c, int len, float a, float
   const T x[4] = {(T)a, (T)b, (T)e, (T)f};
   if constexpr (sizeof(T) == 2) { uint2 w; __builtin_memcpy(&w, x, 8); *reinterpret_cast<uint2*>(row + c) = w; }
   else { at_u4 w; __builtin_memcpy(&w, x, 16); *reinterpret_cast<at_u4*>(row + c) = w; }
+}
+
+// ... of the output, and of what its rounding took away
+template <typename T>
+__device__ __forceinline__ void at_store_out(const AttnP& p, int64_t row, int c, float a, float b, float e, float f) {
+  at_store4<T>(reinterpret_cast<T*>(p.o) + row * p.dv, c, p.dv, a, b, e, f);
+  if (p.o_low)
+    at_store4<T>(reinterpret_cast<T*>(p.o_low) + row * p.dv, c, p.dv, a - (float)(T)a, b - (float)(T)b, e - (float)(T)e, f - (float)(T)f);
 }
 
 __device__ __forceinline__ int at_keys(const AttnP& p, int b) { return p.k_lens ? min(max(p.k_lens[b], 0), p.Lk) : p.Lk; }

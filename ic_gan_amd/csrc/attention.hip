@@ -94,15 +94,15 @@ extern "C" size_t icg_attention_bwd_workspace_bytes(int B, int Lq, int Lk, int H
   return at_bwd_bytes(p, pk);
 }
 
-extern "C" int icg_attention_fwd(const void* q, const void* k, const void* v, const int* k_lens, const int* q_start, void* o, float* lse, int B,
-                                 int Lq, int Lk, int H, int Hk, int d, int dv, int64_t q_sb, int64_t q_sl, int64_t q_sh, int64_t k_sb,
-                                 int64_t k_sl, int64_t k_sh, int64_t v_sb, int64_t v_sl, int64_t v_sh, float scale, int causal, int dtype,
+extern "C" int icg_attention_fwd(const void* q, const void* k, const void* v, const int* k_lens, const int* q_start, void* o, void* o_low,
+                                 float* lse, int B, int Lq, int Lk, int H, int Hk, int d, int dv, int64_t q_sb, int64_t q_sl, int64_t q_sh,
+                                 int64_t k_sb, int64_t k_sl, int64_t k_sh, int64_t v_sb, int64_t v_sl, int64_t v_sh, float scale, int causal, int dtype,
                                  void* workspace, size_t workspace_bytes, void* stream) {
   ICG_REQUIRE(q && k && v && o && lse && at_shape_ok(B, Lq, Lk, H, Hk, d, dv, dtype));
-  ICG_REQUIRE(scale > 0.f && scale < INFINITY && ((uintptr_t)o % 16) == 0);
+  ICG_REQUIRE(scale > 0.f && scale < INFINITY && ((uintptr_t)o % 16) == 0 && ((uintptr_t)o_low % 16) == 0);
   const int size = dtype == 0 ? 4 : 2;
   AttnP p = {};
-  p.q = q, p.k = k, p.v = v, p.k_lens = k_lens, p.q_start = q_start, p.o = o, p.lse = lse;
+  p.q = q, p.k = k, p.v = v, p.k_lens = k_lens, p.q_start = q_start, p.o = o, p.o_low = o_low, p.lse = lse;
   p.B = B, p.Lq = Lq, p.Lk = Lk, p.H = H, p.G = H / Hk, p.d = d, p.dv = dv;
   p.q_sb = q_sb, p.q_sl = q_sl, p.q_sh = q_sh, p.k_sb = k_sb, p.k_sl = k_sl, p.k_sh = k_sh, p.v_sb = v_sb, p.v_sl = v_sl, p.v_sh = v_sh;
   p.scale = scale, p.causal = causal != 0;
@@ -119,19 +119,21 @@ extern "C" int icg_attention_fwd(const void* q, const void* k, const void* v, co
   return dtype == 0 ? at_fwd_f32(p, tok, st) : dtype == 1 ? at_fwd_f16(p, tok, st) : at_fwd_bf16(p, tok, st);
 }
 
-extern "C" int icg_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, const int* k_lens,
+extern "C" int icg_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low, const void* dout,
+                                 const float* lse, const int* k_lens,
                                  const int* q_start, void* dq, void* dk, void* dv_out, int B, int Lq, int Lk, int H, int Hk, int d, int dv,
                                  int64_t q_sb, int64_t q_sl, int64_t q_sh, int64_t k_sb, int64_t k_sl, int64_t k_sh, int64_t v_sb, int64_t v_sl,
                                  int64_t v_sh, int64_t do_sb, int64_t do_sl, int64_t do_sh, float scale, int causal, int dtype, void* workspace,
                                  size_t workspace_bytes, void* stream) {
   ICG_REQUIRE(q && k && v && o && dout && lse && dq && dk && dv_out && at_shape_ok(B, Lq, Lk, H, Hk, d, dv, dtype));
   ICG_REQUIRE(scale > 0.f && scale < INFINITY);
-  ICG_REQUIRE(((uintptr_t)o % 16) == 0 && ((uintptr_t)dq % 16) == 0 && ((uintptr_t)dk % 16) == 0 && ((uintptr_t)dv_out % 16) == 0);
+  ICG_REQUIRE(((uintptr_t)o % 16) == 0 && ((uintptr_t)dq % 16) == 0 && ((uintptr_t)dk % 16) == 0 && ((uintptr_t)dv_out % 16) == 0 &&
+              ((uintptr_t)o_low % 16) == 0);
   if (workspace_bytes < icg_attention_bwd_workspace_bytes(B, Lq, Lk, H, Hk, d, dv, causal, dtype)) return ICG_ERR_WORKSPACE;
   ICG_REQUIRE(workspace && ((uintptr_t)workspace % 16) == 0);
   const int size = dtype == 0 ? 4 : 2;
   AttnP p = {};
-  p.q = q, p.k = k, p.v = v, p.k_lens = k_lens, p.q_start = q_start, p.o = const_cast<void*>(o), p.lse = const_cast<float*>(lse), p.dout = dout;
+  p.q = q, p.k = k, p.v = v, p.k_lens = k_lens, p.q_start = q_start, p.o = const_cast<void*>(o), p.o_low = const_cast<void*>(o_low), p.lse = const_cast<float*>(lse), p.dout = dout;
   p.dq = dq, p.dk = dk, p.dv_out = dv_out;
   p.B = B, p.Lq = Lq, p.Lk = Lk, p.H = H, p.G = H / Hk, p.d = d, p.dv = dv;
   p.q_sb = q_sb, p.q_sl = q_sl, p.q_sh = q_sh, p.k_sb = k_sb, p.k_sl = k_sl, p.k_sh = k_sh, p.v_sb = v_sb, p.v_sl = v_sl, p.v_sh = v_sh;

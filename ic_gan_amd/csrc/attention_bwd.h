@@ -8,7 +8,8 @@
 // (765 TFLOP/s); 64 x 4096 queries, 1024 keys, 24 / 96 elements, fp32: 39, 1130 (114), -, 705 us (109 TFLOP/s).  Bound like the forward kernel by
 // products plus vector instructions of a SIMD, one after the other.
 
-// D_i = do_i . o_i, |do_i| and the exponent's offset; `lanes` lanes (the power of two that covers a row's 16-byte chunks) to a row, rows in
+// D_i = do_i . o_i, |do_i| and the exponent's offset; o_i as it was before its rounding to 16 bits where the forward kept the rest (dp - D
+// cancels: with the rounded o, a row of few keys had twice the error of its products' operands); `lanes` lanes (the power of two that covers a row's 16-byte chunks) to a row, rows in
 // memory order
 template <typename T>
 __global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, float* stat, int lanes) {
@@ -23,11 +24,15 @@ __global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, flo
   if (l * PER < p.dv) {
     const at_u4 a = *reinterpret_cast<const at_u4*>(reinterpret_cast<const T*>(p.o) + i * p.dv + l * PER);
     const at_u4 e = *reinterpret_cast<const at_u4*>(reinterpret_cast<const T*>(p.dout) + b * p.do_sb + qi * p.do_sl + hq * p.do_sh + l * PER);
-    T x[PER], y[PER];
+    T x[PER], y[PER], z[PER] = {};
+    if (p.o_low) {
+      const at_u4 r = *reinterpret_cast<const at_u4*>(reinterpret_cast<const T*>(p.o_low) + i * p.dv + l * PER);
+      __builtin_memcpy(z, &r, 16);
+    }
     __builtin_memcpy(x, &a, 16);
     __builtin_memcpy(y, &e, 16);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) dot = __builtin_fmaf((float)x[j], (float)y[j], dot), sq = __builtin_fmaf((float)y[j], (float)y[j], sq);
+    for (int j = 0; j < PER; ++j) dot = __builtin_fmaf((float)x[j] + (float)z[j], (float)y[j], dot), sq = __builtin_fmaf((float)y[j], (float)y[j], sq);
   }
   for (int s = lanes >> 1; s > 0; s >>= 1) dot += __shfl_xor(dot, s, 64), sq += __shfl_xor(sq, s, 64);
   if (l == 0) {

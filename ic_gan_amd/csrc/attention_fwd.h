@@ -235,13 +235,13 @@ __global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS), (at_fwd_shape<T
   }
   if (writes_stat) p.lse[row] = sum == 0.f ? -INFINITY : mx * AT_LN2 + __logf(sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;        // a row that sees no key is zero
-  T* out = reinterpret_cast<T*>(p.o) + (((int64_t)b * p.Lq + qi) * p.H + hq) * p.dv;
+  const int64_t out = ((int64_t)b * p.Lq + qi) * p.H + hq;
 #pragma unroll
   for (int c = 0; c < NV; ++c)
     if (!TOKENS || c % S::WAVES == wv)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        at_store4<T>(out, 32 * c + 8 * g + 4 * h, p.dv, o[c][4 * g] * inv, o[c][4 * g + 1] * inv, o[c][4 * g + 2] * inv, o[c][4 * g + 3] * inv);
+        at_store_out<T>(p, out, 32 * c + 8 * g + 4 * h, o[c][4 * g] * inv, o[c][4 * g + 1] * inv, o[c][4 * g + 2] * inv, o[c][4 * g + 3] * inv);
 }
 
 // joins the splits of a row: a wave per row, 4 columns a lane, splits in order (one pass over the partial sums)
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256) void icg_attention_join_kernel(AttnP p) {
   if (lane == 0) p.lse[row] = sum == 0.f ? -INFINITY : mx * AT_LN2 + __logf(sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t bh = row / p.Lq, qi = row - bh * p.Lq, b = bh / p.H, hq = bh - b * p.H;
-  at_store4<T>(reinterpret_cast<T*>(p.o) + ((b * p.Lq + qi) * p.H + hq) * p.dv, c, p.dv, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  at_store_out<T>(p, (b * p.Lq + qi) * p.H + hq, c, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
 template <typename T>

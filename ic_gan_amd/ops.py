@@ -1369,8 +1369,8 @@ def _check_index_vector(name, t, B, like):
     return t.contiguous()
 
 
-def _attention_forward(q, k, v, k_lens, q_start, scale, causal):
-    """-> (o, lse) and what the backward pass needs"""
+def _attention_forward(q, k, v, k_lens, q_start, scale, causal, keep=False):
+    """-> (o, lse) and, with `keep`, what the backward pass needs"""
     B, Lq, H, d = q.shape
     Lk, Hk, dv0 = k.shape[1], k.shape[2], v.shape[3]
     dt, per = _DTYPE_CODES[q.dtype], 16 // q.element_size()
@@ -1380,25 +1380,26 @@ def _attention_forward(q, k, v, k_lens, q_start, scale, causal):
     v, sv = _rows_readable(v, dv)
     dev = q.device
     o = torch.empty((B, Lq, H, dv), device=dev, dtype=q.dtype)
+    low = torch.empty_like(o) if keep and q.dtype != torch.float32 else None       # what the rounding of o takes away
     lse = torch.empty((B, H, Lq), device=dev, dtype=torch.float32)
     if B * Lq * H == 0 or Lk == 0:
         o.zero_()
         lse.fill_(float("-inf"))
     else:
         nb = _host_plan("icg_attention_fwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, dt)
-        L.call("icg_attention_fwd", q, k, v, k_lens, q_start, o, lse, B, Lq, Lk, H, Hk, d, dv, *sq, *sk, *sv, scale, int(causal), dt,
+        L.call("icg_attention_fwd", q, k, v, k_lens, q_start, o, low, lse, B, Lq, Lk, H, Hk, d, dv, *sq, *sk, *sv, scale, int(causal), dt,
                _bytes(nb, dev) if nb else None, nb)
-    return (o if dv == dv0 else o[..., :dv0].contiguous()), lse, (q, k, v, o)
+    return (o if dv == dv0 else o[..., :dv0].contiguous()), lse, (q, k, v, o, low)
 
 
 class AttentionFn(Function):
-    """Forward: output and log-sum-exp only (icg_attention_fwd).  Backward: the probabilities again, tile by tile (icg_attention_bwd);
+    """Forward: output (16-bit types: and what its rounding took away) and log-sum-exp only (icg_attention_fwd).  Backward: the probabilities again, tile by tile (icg_attention_bwd);
     fixed summation order, no atomics."""
 
     @staticmethod
     def forward(ctx, q, k, v, k_lens, q_start, scale, causal):
         ctx.widths, ctx.scale, ctx.causal = (q.shape[3], v.shape[3]), scale, causal
-        o, lse, kept = _attention_forward(q, k, v, k_lens, q_start, scale, causal)
+        o, lse, kept = _attention_forward(q, k, v, k_lens, q_start, scale, causal, keep=True)
         ctx.save_for_backward(*kept, lse, k_lens, q_start)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)               # (no tensor of zeros for lse)
@@ -1409,7 +1410,7 @@ class AttentionFn(Function):
     def backward(ctx, do, dlse=None):
         if do is None:
             return (None,) * 7
-        q, k, v, o, lse, k_lens, q_start = ctx.saved_tensors
+        q, k, v, o, low, lse, k_lens, q_start = ctx.saved_tensors
         B, Lq, H, d = q.shape
         Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
         dt, dev = _DTYPE_CODES[q.dtype], q.device
@@ -1419,7 +1420,7 @@ class AttentionFn(Function):
         else:
             do, sdo = _rows_readable(do, dv)
             nb = _host_plan("icg_attention_bwd_workspace_bytes", B, Lq, Lk, H, Hk, d, dv, int(ctx.causal), dt)
-            L.call("icg_attention_bwd", q, k, v, o, do, lse, k_lens, q_start, dq, dk, dv_, B, Lq, Lk, H, Hk, d, dv, *q.stride()[:3], *k.stride()[:3],
+            L.call("icg_attention_bwd", q, k, v, o, low, do, lse, k_lens, q_start, dq, dk, dv_, B, Lq, Lk, H, Hk, d, dv, *q.stride()[:3], *k.stride()[:3],
                    *v.stride()[:3], *sdo, ctx.scale, int(ctx.causal), dt, _bytes(nb, dev), nb)
         if ctx.widths != (d, dv):
             dq, dk, dv_ = dq[..., :ctx.widths[0]], dk[..., :ctx.widths[0]], dv_[..., :ctx.widths[1]]

@@ -790,18 +790,20 @@ int icg_sg2_torgb_bwd(const float* dimg, const void* y, const void* x, const flo
  * and its gradient, which computes the probabilities again from q, k and l.  q [B][Lq][H][d], k [B][Lk][Hk][d], v [B][Lk][Hk][dv] with the
  * given element strides of batch, position and head (last dimension contiguous; rows are whole 16-byte chunks at multiples of 16 bytes,
  * positions at least a row and less than 16 MB apart; heads and batches may overlap); query head h reads key head h / (H / Hk).  o, dq [B][Lq][H][..], dk, dv_out [B][Lk][Hk][..] contiguous, 16-byte aligned; lse [B][H][Lq] fp32.
+ * o_low, like o, or NULL: what the rounding of o to 16 bits took away, for the gradient's row sums do . o (without it they are those of the
+ * rounded o).
  * dtype 0 / 1 / 2: fp32 / fp16 / bf16 (matrix products in that type, everything else in fp32).  k_lens, q_start: int32 [B] on the device or
  * NULL (Lk; Lk - Lq); keys from k_lens[b] on are not read, and their dk, dv are zero.  scale > 0.  `_applies`: d, dv <= 128, or d <= 64 and
  * dv <= 256, rows of whole 16-byte chunks.  A non-finite value that the causal mask hides from a query can still reach it (0 * inf); one from k_lens[b] on cannot. */
 int icg_attention_applies(int B, int Lq, int Lk, int H, int Hk, int d, int dv, int dtype);
 size_t icg_attention_fwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hk, int d, int dv, int dtype);
-int icg_attention_fwd(const void* q, const void* k, const void* v, const int* k_lens, const int* q_start, void* o, float* lse, int B, int Lq,
-                      int Lk, int H, int Hk, int d, int dv, int64_t q_sb, int64_t q_sl, int64_t q_sh, int64_t k_sb, int64_t k_sl, int64_t k_sh,
+int icg_attention_fwd(const void* q, const void* k, const void* v, const int* k_lens, const int* q_start, void* o, void* o_low, float* lse,
+                      int B, int Lq, int Lk, int H, int Hk, int d, int dv, int64_t q_sb, int64_t q_sl, int64_t q_sh, int64_t k_sb, int64_t k_sl, int64_t k_sh,
                       int64_t v_sb, int64_t v_sl, int64_t v_sh, float scale, int causal, int dtype, void* workspace, size_t workspace_bytes,
                       void* stream);
 size_t icg_attention_bwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hk, int d, int dv, int causal, int dtype);
-int icg_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, const int* k_lens,
-                      const int* q_start, void* dq, void* dk, void* dv_out, int B, int Lq, int Lk, int H, int Hk, int d, int dv, int64_t q_sb,
+int icg_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low, const void* dout, const float* lse,
+                      const int* k_lens, const int* q_start, void* dq, void* dk, void* dv_out, int B, int Lq, int Lk, int H, int Hk, int d, int dv, int64_t q_sb,
                       int64_t q_sl, int64_t q_sh, int64_t k_sb, int64_t k_sl, int64_t k_sh, int64_t v_sb, int64_t v_sl, int64_t v_sh,
                       int64_t do_sb, int64_t do_sl, int64_t do_sh, float scale, int causal, int dtype, void* workspace, size_t workspace_bytes,
                       void* stream);

@@ -1557,18 +1557,22 @@ def _attention_probabilities(q, k, v, k_lens, q_start, Hk, scale, causal):
     return Q, K, V, torch.exp(s - lse.unsqueeze(-1).nan_to_num(neginf=0.0)), lse
 
 
-def icg_attention_fwd(q, k, v, k_lens, q_start, o, lse, B, Lq, Lk, H, Hk, d, dv, *rest):
+def icg_attention_fwd(q, k, v, k_lens, q_start, o, o_low, lse, B, Lq, Lk, H, Hk, d, dv, *rest):
     scale, causal = rest[9], rest[10]
     _, _, V, p, l = _attention_probabilities(q, k, v, k_lens, q_start, Hk, scale, causal)
-    o.copy_((p @ V).transpose(1, 2))
+    exact = (p @ V).transpose(1, 2)
+    o.copy_(exact)
+    if o_low is not None:
+        o_low.copy_(exact - o.float())
     lse.copy_(l)
 
 
-def icg_attention_bwd(q, k, v, o, dout, lse, k_lens, q_start, dq, dk, dv_out, B, Lq, Lk, H, Hk, d, dv, *rest):
+def icg_attention_bwd(q, k, v, o, o_low, dout, lse, k_lens, q_start, dq, dk, dv_out, B, Lq, Lk, H, Hk, d, dv, *rest):
     scale, causal = rest[12], rest[13]
     Q, K, V, p, _ = _attention_probabilities(q, k, v, k_lens, q_start, Hk, scale, causal)
     dO = dout.detach().float().transpose(1, 2)
-    ds = p * (dO @ V.transpose(-1, -2) - (dO * o.float().transpose(1, 2)).sum(-1, keepdim=True)) * scale
+    whole = o.float() if o_low is None else o.float() + o_low.float()
+    ds = p * (dO @ V.transpose(-1, -2) - (dO * whole.transpose(1, 2)).sum(-1, keepdim=True)) * scale
     shared = lambda t: t.reshape(B, Hk, H // Hk, Lk, -1).sum(2).transpose(1, 2)
     dq.copy_((ds @ K).transpose(1, 2))
     dk.copy_(shared(ds.transpose(-1, -2) @ Q))

@@ -75,11 +75,11 @@ def test_entry_points_refuse_before_a_launch():
     lib = _lib.lib()
     buf = ctypes.create_string_buffer(4096)
     p = (ctypes.addressof(buf) + 15) & ~15
-    def fwd(q=p, o=p, B=1, Lq=1, Lk=2048, H=2, Hk=1, d=8, dv=8, scale=1.0, dtype=0, ws=p, nb=0):
-        return lib.icg_attention_fwd(q, p, p, None, None, o, p, B, Lq, Lk, H, Hk, d, dv, *[8] * 9, scale, 0, dtype, ws, nb, None)
-    assert fwd(q=None) == -1 and fwd(o=p + 4) == -1 and fwd(Hk=3) == -1 and fwd(d=200) == -1 and fwd(d=128, dv=256) == -1
+    def fwd(q=p, o=p, o_low=None, B=1, Lq=1, Lk=2048, H=2, Hk=1, d=8, dv=8, scale=1.0, dtype=0, ws=p, nb=0):
+        return lib.icg_attention_fwd(q, p, p, None, None, o, o_low, p, B, Lq, Lk, H, Hk, d, dv, *[8] * 9, scale, 0, dtype, ws, nb, None)
+    assert fwd(q=None) == -1 and fwd(o=p + 4) == -1 and fwd(o_low=p + 8) == -1 and fwd(Hk=3) == -1 and fwd(d=200) == -1 and fwd(d=128, dv=256) == -1
     assert fwd(scale=0.0) == -1 and fwd(scale=float("nan")) == -1 and fwd(dtype=3) == -1 and fwd(Lq=0) == -1 and fwd(B=1 << 20, H=1 << 12) == -1
     assert lib.icg_attention_fwd_workspace_bytes(1, 1, 2048, 2, 1, 8, 8, 0) > 0 and fwd(nb=0) == -3
     def bwd(dq=p, nb=1 << 20, Lq=1, ws=p):
-        return lib.icg_attention_bwd(p, p, p, p, p, p, None, None, dq, p, p, 1, Lq, 16, 2, 1, 8, 8, *[8] * 12, 1.0, 0, 0, ws, nb, None)
+        return lib.icg_attention_bwd(p, p, p, p, None, p, p, None, None, dq, p, p, 1, Lq, 16, 2, 1, 8, 8, *[8] * 12, 1.0, 0, 0, ws, nb, None)
     assert bwd(dq=None) == -1 and bwd(dq=p + 8) == -1 and bwd(nb=0) == -3 and bwd(ws=None) == -1 and bwd(Lq=-1) == -1
