@@ -4,7 +4,7 @@
 #pragma once
 #include "attention.h"
 
-// Measured, 2 x 4096 causal, 16 heads of 128 over 4 key heads, bf16: row sums 16 us, dk and dv 375 us (735 TFLOP/s), their join 14 us, dq 270 us
+// Measured, 2 x 4096 causal, 16 heads of 128 over 4 key heads, bf16: row sums 23 us, dk and dv 373 us (740 TFLOP/s), their join 14 us, dq 270 us
 // (765 TFLOP/s); 64 x 4096 queries, 1024 keys, 24 / 96 elements, fp32: 39, 1130 (114), -, 705 us (109 TFLOP/s).  Bound like the forward kernel by
 // products plus vector instructions of a SIMD, one after the other.
 
