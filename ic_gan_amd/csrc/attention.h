@@ -48,7 +48,7 @@ struct AttnP {
   // gradient
   const void* dout;
   int64_t do_sb, do_sl, do_sh;
-  const float *stat;                        // [3][B][H][Lq]: l_i log2 e (less the shift of p), D_i, |do_i|
+  const float *stat;                        // [3][B][H][Lq]: l_i log2 e (less the shift of p), D_i, |do_i|; SCALED: then [B][Hk][ceil(Lk / 128)]: largest |v_j|
   void *dq, *dk, *dv_out;
   int tiles;                                // 32- or 128-row tiles of one head
   int64_t work;                             // workgroups in all
@@ -85,9 +85,10 @@ template <> struct at_type<__bf16> {
     return f;
   }
 };
-// 16-bit floats end at 6e-8: in the gradient p is held 2^6 times as large, and ds is scaled by a power of two that brings the largest |do|
-// to [1, 2) (undone on the 32-bit sums, exactly), so that gradients of a mean over many pixels do not vanish.  |p (dp - D)| <= |do| |v| / 2,
-// so ds stays below 65504 for |v| up to 1000; it is clamped there.
+// fp16 ends at 6e-8 and at 65504: in the gradient p is held 2^6 times as large, and ds is scaled by a power of two (undone on the 32-bit
+// sums, exactly).  |p_j (do . v_j - do . o)| = p_j |sum_k p_k do . (v_j - v_k)| <= p_j (1 - p_j) |do| 2 max|v| <= |do| max|v| / 2, so the power
+// that brings |do| max|v| to [512, 1024) holds ds below 2^15 for any values that the type has, with a factor of 2 to spare for the roundings
+// of p and D; what is lost below is half of 2^-24 in that scale, 2^-40 |do| max|v|.
 template <> struct at_type<_Float16> {
   typedef at_h8 frag;
   static constexpr int KSTEP = 16, P_SHIFT = 6;

@@ -45,11 +45,15 @@ void at_plan_dkv(AttnP& p) {
   p.nsplit = (int)(n > 1 ? n : 1);
   p.work = items * p.nsplit;
 }
-size_t at_stat_bytes(const AttnP& p) { return ((size_t)3 * p.B * p.H * p.Lq * 4 + 15) / 16 * 16; }
-size_t at_bwd_bytes(const AttnP& dq, const AttnP& dkv) {
+// three numbers a query, and for fp16 one for every 128 keys
+size_t at_stat_bytes(const AttnP& p, int dtype) {
+  const size_t keys = dtype == 1 ? (size_t)p.B * (p.H / p.G) * icg_cdiv(p.Lk, 128) : 0;
+  return (((size_t)3 * p.B * p.H * p.Lq + keys) * 4 + 15) / 16 * 16;
+}
+size_t at_bwd_bytes(const AttnP& dq, const AttnP& dkv, int dtype) {
   const size_t a = dq.nsplit > 1 ? (size_t)dq.nsplit * dq.B * dq.H * dq.Lq * dq.d * 4 : 0;
   const size_t b = dkv.nsplit > 1 ? (size_t)dkv.nsplit * dkv.B * dkv.Lk * (dkv.H / dkv.G) * (dkv.d + dkv.dv) * 4 : 0;
-  return at_stat_bytes(dq) + (a > b ? a : b);
+  return at_stat_bytes(dq, dtype) + (a > b ? a : b);
 }
 
 size_t at_part_bytes(const AttnP& p) {
@@ -91,7 +95,7 @@ extern "C" size_t icg_attention_bwd_workspace_bytes(int B, int Lq, int Lk, int H
   AttnP pk = p;
   at_plan_dq(p);
   at_plan_dkv(pk);
-  return at_bwd_bytes(p, pk);
+  return at_bwd_bytes(p, pk, dtype);
 }
 
 extern "C" int icg_attention_fwd(const void* q, const void* k, const void* v, const int* k_lens, const int* q_start, void* o, void* o_low,
@@ -142,7 +146,7 @@ extern "C" int icg_attention_bwd(const void* q, const void* k, const void* v, co
   ICG_REQUIRE(at_row_ok(q, q_sb, q_sl, q_sh, d, size) && at_row_ok(k, k_sb, k_sl, k_sh, d, size) && at_row_ok(v, v_sb, v_sl, v_sh, dv, size));
   ICG_REQUIRE(at_row_ok(dout, do_sb, do_sl, do_sh, dv, size));
   float* stat = (float*)workspace;
-  p.part = (float*)((char*)workspace + at_stat_bytes(p));
+  p.part = (float*)((char*)workspace + at_stat_bytes(p, dtype));
   AttnP pk = p;
   at_plan_dq(p);
   at_plan_dkv(pk);

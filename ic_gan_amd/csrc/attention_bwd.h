@@ -10,16 +10,42 @@
 
 // D_i = do_i . o_i, |do_i| and the exponent's offset; o_i as it was before its rounding to 16 bits where the forward kept the rest (dp - D
 // cancels: with the rounded o, a row of few keys had twice the error of its products' operands); `lanes` lanes (the power of two that covers a row's 16-byte chunks) to a row, rows in
-// memory order
+// memory order.  SCALED: the workgroups from `row_blocks` on take 128 keys of a key head each and find their largest |v_j| (finite ones: a row
+// that sees another has no finite gradient anyhow)
 template <typename T>
-__global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, float* stat, int lanes) {
+__global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, float* stat, int lanes, unsigned row_blocks) {
+  constexpr int PER = 16 / (int)sizeof(T);
   const int64_t rows = (int64_t)p.B * p.H * p.Lq, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
   const int l = threadIdx.x & (lanes - 1);
+  if constexpr (at_type<T>::SCALED) {
+    if (blockIdx.x >= row_blocks) {
+      __shared__ float red[4];
+      const int64_t item = blockIdx.x - row_blocks, tiles = (p.Lk + 127) / 128, bh = item / tiles;
+      const int Hk = p.H / p.G, b = (int)(bh / Hk), hk = (int)(bh - (int64_t)b * Hk), tile = (int)(item - bh * tiles), keys = at_keys(p, b);
+      float most = 0.f;
+      for (int j = 128 * tile + (int)threadIdx.x / lanes; j < min(keys, 128 * tile + 128); j += 256 / lanes) {
+        float sq = 0.f;
+        if (l * PER < p.dv) {
+          const at_u4 a = *reinterpret_cast<const at_u4*>(reinterpret_cast<const T*>(p.v) + b * p.v_sb + j * p.v_sl + hk * p.v_sh + l * PER);
+          T x[PER];
+          __builtin_memcpy(x, &a, 16);
+#pragma unroll
+          for (int e = 0; e < PER; ++e) sq = __builtin_fmaf((float)x[e], (float)x[e], sq);
+        }
+        for (int s = lanes >> 1; s > 0; s >>= 1) sq += __shfl_xor(sq, s, 64);
+        most = fmaxf(most, __builtin_isfinite(sq) ? sq : 0.f);
+      }
+      most = wave_max(most);
+      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+      __syncthreads();
+      if (threadIdx.x == 0) stat[3 * rows + item] = sqrtf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+      return;
+    }
+  }
   if (i >= rows) return;
   const int64_t bq = i / p.H;
   const int hq = (int)(i - bq * p.H);
   const int64_t b = bq / p.Lq, qi = bq - b * p.Lq;
-  constexpr int PER = 16 / (int)sizeof(T);
   float dot = 0.f, sq = 0.f;
   if (l * PER < p.dv) {
     const at_u4 a = *reinterpret_cast<const at_u4*>(reinterpret_cast<const T*>(p.o) + i * p.dv + l * PER);
@@ -49,12 +75,27 @@ __device__ __forceinline__ float at_to_one(float norm) {
   const unsigned e = (__float_as_uint(norm) >> 23) & 255u;
   return e == 0u || e >= 254u ? 1.f : __uint_as_float((254u - e) << 23);
 }
-template <typename T>
-__device__ __forceinline__ float at_ds(float pr, float dp, float s, float delta_s) {
-  const float x = pr * __builtin_fmaf(dp, s, -delta_s);
-  if constexpr (at_type<T>::SCALED) return __builtin_isfinite(x) ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x;      // (inf and NaN stay visible)
-  return x;
+// the power of two that ds of rows with |do| <= g is held by
+__device__ __forceinline__ float at_ds_scale(float g, float vmax) { return 512.f * at_to_one(g * vmax); }
+__device__ __forceinline__ float at_finite(float x) { return __builtin_isfinite(x) ? x : 0.f; }
+// the largest of each thread's n, for all 256 threads (red: 4 floats of LDS, free again on return)
+__device__ __forceinline__ float at_block_max(float n, float* red) {
+  n = wave_max(n);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
+  __syncthreads();
+  n = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  __syncthreads();
+  return n;
 }
+// the largest |v_j| of a key head (SCALED)
+__device__ __forceinline__ float at_vmax(const AttnP& p, int b, int hk, int64_t rows, float* red) {
+  const int tiles = (p.Lk + 127) / 128;
+  const float* of = p.stat + 3 * rows + ((int64_t)b * (p.H / p.G) + hk) * tiles;
+  float n = 0.f;
+  for (int i = threadIdx.x; i < tiles; i += 256) n = fmaxf(n, of[i]);
+  return at_block_max(n, red);
+}
+__device__ __forceinline__ float at_ds(float pr, float dp, float s, float delta_s) { return pr * __builtin_fmaf(dp, s, -delta_s); }
 
 // dq: a workgroup owns 128 queries of one head (a wave 32, as columns) and streams the keys, or its split of them
 template <typename T, int DP, int DVP> constexpr int at_dq_waves() { return (DP + DVP) * (int)sizeof(T) / 8 + DP / 2 <= 144 ? 2 : 1; }
@@ -86,7 +127,11 @@ __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attentio
   at_own<T, DVP>(gf, reinterpret_cast<const T*>(p.dout) + b * p.do_sb + qi * p.do_sl + hq * p.do_sh, valid, p.dv, h);
   const int64_t rows = (int64_t)p.B * p.H * p.Lq, row = ((int64_t)b * p.H + hq) * p.Lq + qi;
   const float lse2 = valid ? p.stat[row] : INFINITY;
-  const float s1 = X::SCALED && valid ? at_to_one(p.stat[2 * rows + row]) : 1.f;
+  float s1 = 1.f;
+  if constexpr (X::SCALED) {
+    const float vmax = at_vmax(p, b, hk, rows, reinterpret_cast<float*>(lds));
+    s1 = valid ? at_ds_scale(p.stat[2 * rows + row], vmax) : 1.f;
+  }
   const float delta = valid ? p.stat[rows + row] * s1 : 0.f;
   const at_rows kb(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_sl, p.d, sizeof(T));
   const at_rows vb(reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_sl, p.dv, sizeof(T));
@@ -130,7 +175,7 @@ __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attentio
 #pragma unroll
       for (int t = 0; t < DVP / X::KSTEP; ++t) dp = X::mma(vr.row_frag(vt, 32 * u, t), gf[t], dp);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = at_ds<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scl, -lse2)), dp[i], s1, delta);
+      for (int i = 0; i < 16; ++i) s[i] = at_ds(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scl, -lse2)), dp[i], s1, delta);
       if (__any(j0 + 32 * u + 31 > last)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = j0 + 32 * u + at_row_of(i, h) > last ? 0.f : s[i];
@@ -210,12 +255,9 @@ __global__ __launch_bounds__(256, (at_dkv_shape<T, DP, DVP>::WAVES)) void icg_at
   if constexpr (X::SCALED) {                             // one scale for everything that is summed here
     float* red = reinterpret_cast<float*>(lds);
     float n = 0.f;
-    for (int64_t i = tid; i < (int64_t)p.G * p.Lq; i += 256) n = fmaxf(n, p.stat[2 * rows + row_b + i]);
-    n = wave_max(n);
-    if (lane == 0) red[wv] = n;
-    __syncthreads();
-    s1 = at_to_one(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    __syncthreads();
+    for (int64_t i = tid; i < (int64_t)p.G * p.Lq; i += 256) n = fmaxf(n, at_finite(p.stat[2 * rows + row_b + i]));
+    n = at_block_max(n, red);
+    s1 = at_ds_scale(n, at_vmax(p, b, hk, rows, red));
   }
 
   at_f16v dk[DP / 32], dv[DVP / 32];
@@ -290,7 +332,7 @@ __global__ __launch_bounds__(256, (at_dkv_shape<T, DP, DVP>::WAVES)) void icg_at
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * g + e;
           s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scl, -l4[e]));
-          dp[i] = at_ds<T>(s[i], dp[i], s1, d4[e]);
+          dp[i] = at_ds(s[i], dp[i], s1, d4[e]);
         }
       }
       if (edge) {
@@ -383,7 +425,9 @@ int at_bwd(AttnP p, AttnP pk, float* stat, hipStream_t st) {
   p.stat = pk.stat = stat;
   int lanes = 1;
   while (lanes * 16 < p.dv * (int)sizeof(T)) lanes <<= 1;        // (at most 64: rows of up to 256 fp32)
-  hipLaunchKernelGGL((icg_attention_rowstat_kernel<T>), dim3((unsigned)icg_cdiv((int64_t)p.B * p.H * p.Lq * lanes, 256)), dim3(256), 0, st, p, stat, lanes);
+  const int64_t row_blocks = icg_cdiv((int64_t)p.B * p.H * p.Lq * lanes, 256);
+  const int64_t key_blocks = at_type<T>::SCALED ? (int64_t)p.B * (p.H / p.G) * icg_cdiv(p.Lk, 128) : 0;
+  hipLaunchKernelGGL((icg_attention_rowstat_kernel<T>), dim3((unsigned)(row_blocks + key_blocks)), dim3(256), 0, st, p, stat, lanes, (unsigned)row_blocks);
   if (const int e = icg_check_launch()) return e;
 #define AT_RUN(DP, DVP)                                                                                                  \
   do {                                                                                                                   \
