@@ -48,10 +48,11 @@ __device__ __forceinline__ void gn_store(T* p, const gn_vec<T, VEC>& r) {
 }
 
 __device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f)); }
-__device__ __forceinline__ float gn_act(float z, int act) { return act == 0 ? z : act == 1 ? fmaxf(z, 0.f) : z * gn_sigmoid(z); }
+// (a comparison and not a maximum, which would turn NaN into 0: a group with a value that is not finite shows it after a ReLU too)
+__device__ __forceinline__ float gn_act(float z, int act) { return act == 0 ? z : act == 1 ? (z < 0.f ? 0.f : z) : z * gn_sigmoid(z); }
 __device__ __forceinline__ float gn_dact(float z, int act) {
   if (act == 0) return 1.f;
-  if (act == 1) return z > 0.f ? 1.f : 0.f;
+  if (act == 1) return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;      // (NaN stays)
   const float s = gn_sigmoid(z);
   return s * (1.f + z * (1.f - s));
 }

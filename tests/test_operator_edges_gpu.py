@@ -71,3 +71,50 @@ def test_fp16_gradients_of_large_values(name, up, lone):
     for n, got, more in (("o", o, None), ("dq", dq, more_q), ("dk", dk, more_k), ("dv", dv, None)):
         value, bound = want[n]
         A.check(got, (value, bound if more is None else bound + more.transpose(1, 2)), n)
+
+
+# ---- group norm of non-finite values ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")], ids=["nan", "inf", "-inf"])
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+@pytest.mark.parametrize("shape,groups", [((2, 48, 7, 5), 16), ((2, 64, 40, 48), 4), ((2, 96, 96, 80), 16), ((1, 33, 101, 97), 3)],
+                         ids=["one_pass", "one_pass_wide", "three_passes", "three_passes_scalar"])
+def test_norm_shows_what_is_not_finite(shape, groups, dtype, act, bad):
+    """one NaN or infinity makes its group's mean and deviation NaN, and so every value and gradient of that group and sample, whatever the
+    activation; no other group, and no other sample, changes"""
+    from ic_gan_amd import ops
+    g = torch.Generator().manual_seed(3)
+    B, C, H, W = shape
+    x, dy = (torch.randn(*shape, generator=g).to(dtype).cuda().contiguous(memory_format=torch.channels_last) for _ in range(2))
+    gain, bias = (torch.randn(B, C, generator=g).cuda() for _ in range(2))
+    runs = []
+    for value in (None, bad):
+        leaves = [x.clone(), gain.clone(), bias.clone()]
+        if value is not None:
+            leaves[0][B - 1, C // 2, H // 2, W // 3] = value
+        for t in leaves:
+            t.requires_grad_()
+        y = ops.group_norm_act(leaves[0], groups, leaves[1], leaves[2], act=act)
+        runs.append((y.detach(),) + torch.autograd.grad(y, leaves, dy))
+    at = slice(C // 2 // (C // groups) * (C // groups), (C // 2 // (C // groups) + 1) * (C // groups))
+    for name, a, b in zip(("y", "dx", "dgain", "dbias"), *runs):
+        assert torch.isfinite(a).all()
+        if name != "dbias" or act != "none":                     # (without an activation dbias is the sum of dy, whatever x is)
+            assert torch.isnan(b[B - 1, at]).all(), name
+            b = b.clone()
+            b[B - 1, at] = a[B - 1, at]
+        assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+@pytest.mark.parametrize("shape,groups", [((3, 32, 4, 4), 8), ((2, 96, 96, 80), 16)], ids=["one_pass", "three_passes"])
+def test_norm_shows_a_gain_that_is_not_finite(shape, groups, act):
+    from ic_gan_amd import ops
+    x = torch.randn(*shape, device="cuda").contiguous(memory_format=torch.channels_last)
+    gain, bias = torch.randn(shape[1], device="cuda"), torch.randn(shape[1], device="cuda")
+    good = ops.group_norm_act(x, groups, gain, bias, act=act)
+    gain[3] = float("nan")
+    y = ops.group_norm_act(x, groups, gain, bias, act=act)
+    assert torch.isnan(y[:, 3]).all()
+    y[:, 3] = good[:, 3]
+    assert torch.equal(y, good)
