@@ -14,7 +14,7 @@ from typing import Optional
 
 import torch
 import torch.distributed as dist
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -1334,10 +1334,13 @@ def _rows_readable(t, width):
 
 
 def _first_order(backward):
-    """once_differentiable, without its detour where no second derivative can be asked for (a small call's backward pass is bound by the host)"""
+    """once_differentiable, without its detour where no second derivative can be asked for (a small call's backward pass is bound by the host);
+    a gradient that carries a forward-mode tangent is refused: the kernels would drop it without a word"""
     guarded = once_differentiable(backward)
 
     def run(ctx, *grads):
+        if forward_ad._current_level >= 0 and any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+            raise NotImplementedError("ic_gan_amd: forward-mode derivatives of this operator's backward pass are not implemented")
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 
@@ -1429,7 +1432,7 @@ class AttentionFn(Function):
 
 def attention(q, k, v, *, scale=None, causal=False, k_lens=None, q_start=None, return_lse=False):
     """softmax(scale q k^T) v per head, with the probabilities never in memory: o [B, Lq, H, dv] (and, with `return_lse`, the log of the
-    softmax sums [B, H, Lq], fp32, without gradient).  Differentiable once in q, k and v.
+    softmax sums [B, H, Lq], fp32, without gradient).  Differentiable once in q, k and v, in reverse mode only (a forward-mode tangent is refused).
 
     q [B, Lq, H, d], k [B, Lk, Hk, d], v [B, Lk, Hk, dv]: fp32, fp16 or bf16, any strides; H a multiple of Hk (heads h with the same
     h // (H // Hk) share a key head); d, dv <= 128, or d <= 64 and dv <= 256.
@@ -1462,7 +1465,9 @@ def attention(q, k, v, *, scale=None, causal=False, k_lens=None, q_start=None, r
     if B * Lq * Lk and not _host_plan("icg_attention_applies", B, Lq, Lk, H, Hk, -(-d // 8) * 8, -(-dv // 8) * 8, _DTYPE_CODES[dtype]):
         raise ValueError("attention: not served: B %d, Lq %d, Lk %d, H %d, d %d, dv %d (d, dv <= 128, or d <= 64 and dv <= 256)" % (B, Lq, Lk, H, d, dv))
     _require_gpu(q)
-    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+    # (with forward-mode levels or function transforms about, the call goes by the autograd node, which refuses what it cannot differentiate)
+    plain = forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active()
+    if plain and not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         o, lse, _ = _attention_forward(q, k, v, k_lens, q_start, scale, bool(causal))
         return (o, lse) if return_lse else o
     o, lse = AttentionFn.apply(q, k, v, k_lens, q_start, scale, bool(causal))

@@ -1,0 +1,51 @@
+"""What ops.attention, ops.group_norm_act and ops.embedding refuse at the ends of their ranges, forward-mode derivatives, and the device that a
+kernel is launched on (no GPU: kernels emulated or entry points that check on the host)."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from oracle import kernel_ref
+
+
+def _calls(ops):
+    q, k, v = (torch.randn(2, n, 2, 8) for n in (3, 5, 5))
+    x, gain, bias = torch.randn(2, 8, 3, 3), torch.randn(8), torch.randn(8)
+    w, idx = torch.randn(7, 4), torch.tensor([1, 5, 1])
+    return {"attention": (lambda q, k, v: ops.attention(q, k, v), (q, k, v)),
+            "attention_lse": (lambda q, k, v: ops.attention(q, k, v, return_lse=True)[0], (q, k, v)),
+            "group_norm_act": (lambda x, gain, bias: ops.group_norm_act(x, 2, gain, bias, act="silu"), (x, gain, bias)),
+            "embedding": (lambda w: ops.embedding(idx, w), (w,))}
+
+
+@pytest.mark.parametrize("graph", [False, True], ids=["no_gradient", "gradient"])
+@pytest.mark.parametrize("name", ["attention", "attention_lse", "group_norm_act", "embedding"])
+def test_a_tangent_is_refused_and_not_lost(name, graph, monkeypatch):
+    kernel_ref.install(monkeypatch)
+    from ic_gan_amd import ops
+    f, ins = _calls(ops)[name]
+    want = f(*ins)
+    with forward_ad.dual_level():
+        assert torch.equal(f(*ins), want)                        # (no tangent: an ordinary call)
+        for i in range(len(ins)):
+            dual = [forward_ad.make_dual(t.clone().requires_grad_(graph), torch.ones_like(t)) if j == i else t for j, t in enumerate(ins)]
+            with pytest.raises(NotImplementedError):
+                f(*dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                f(*dual)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(f, ins, tuple(torch.ones_like(t) for t in ins))
+
+
+@pytest.mark.parametrize("name", ["attention", "group_norm_act", "embedding"])
+def test_a_gradient_with_a_tangent_is_refused(name, monkeypatch):
+    kernel_ref.install(monkeypatch)
+    from ic_gan_amd import ops
+    f, ins = _calls(ops)[name]
+    ins = [t.clone().requires_grad_() for t in ins]
+    y = f(*ins)
+    want = torch.autograd.grad(y, ins, torch.ones_like(y), retain_graph=True)
+    with forward_ad.dual_level():
+        for a, b in zip(torch.autograd.grad(y, ins, torch.ones_like(y), retain_graph=True), want):
+            assert torch.equal(a, b)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(y, ins, forward_ad.make_dual(torch.ones_like(y), torch.randn_like(y)))
