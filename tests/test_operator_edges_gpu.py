@@ -73,6 +73,31 @@ def test_fp16_gradients_of_large_values(name, up, lone):
         A.check(got, (value, bound if more is None else bound + more.transpose(1, 2)), n)
 
 
+# ---- keys that no query sees -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")], ids=["nan", "inf"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
+@pytest.mark.parametrize("Lq,d,dv", [(1, 64, 64), (5, 24, 96), (33, 128, 128), (130, 40, 40), (150, 64, 256)])
+def test_what_lies_behind_the_last_query(Lq, d, dv, dtype, bad):
+    """causal with q_start into a longer buffer, as a chunk of a prompt meets a cache: keys behind the last query's own are seen by none, whatever
+    they hold, and their gradient is zero"""
+    from ic_gan_amd import ops
+    B, Lk, H, Hk = 2, 300, 4, 2
+    start = [0, 17]
+    q, k, v, do = (torch.randn(B, n, h, e, device="cuda").to(dtype) for n, h, e in ((Lq, H, d), (Lk, Hk, d), (Lk, Hk, dv), (Lq, H, dv)))
+    runs = []
+    for fill in (0.0, bad):
+        kk, vv = k.clone(), v.clone()
+        for b, s in enumerate(start):
+            kk[b, s + Lq:], vv[b, s + Lq:] = fill, fill
+        leaves = [t.clone().requires_grad_() for t in (q, kk, vv)]
+        o = ops.attention(*leaves, causal=True, q_start=torch.tensor(start, device="cuda", dtype=torch.int32))
+        runs.append((o.detach(),) + torch.autograd.grad(o, leaves, do))
+    for name, a, b in zip(("o", "dq", "dk", "dv"), *runs):
+        assert torch.isfinite(a).all() and torch.equal(a, b), name
+    for b, s in enumerate(start):
+        assert not runs[1][2][b, s + Lq:].any() and not runs[1][3][b, s + Lq:].any()
+
+
 # ---- group norm of non-finite values ---------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")], ids=["nan", "inf", "-inf"])
 @pytest.mark.parametrize("act", ["none", "relu", "silu"])
