@@ -235,9 +235,18 @@ __device__ __forceinline__ void at_store4(T* row, int c, int len, float a, float
   else { at_u4 w; __builtin_memcpy(&w, x, 16); *reinterpret_cast<at_u4*>(row + c) = w; }
 }
 
+// A mean of fp16 values is held to their range: p is rounded for the product with v and not in its sum, so the quotient can pass 65504 by a
+// step of 2^-11, from where a conversion gives inf.  (A sum that is not finite has a value that is not, and stays.)
+template <typename T>
+__device__ __forceinline__ float at_hold(float x) {
+  if constexpr (at_type<T>::SCALED) return __builtin_isfinite(x) ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x;
+  return x;
+}
+
 // ... of the output, and of what its rounding took away
 template <typename T>
 __device__ __forceinline__ void at_store_out(const AttnP& p, int64_t row, int c, float a, float b, float e, float f) {
+  a = at_hold<T>(a), b = at_hold<T>(b), e = at_hold<T>(e), f = at_hold<T>(f);
   at_store4<T>(reinterpret_cast<T*>(p.o) + row * p.dv, c, p.dv, a, b, e, f);
   if (p.o_low)
     at_store4<T>(reinterpret_cast<T*>(p.o_low) + row * p.dv, c, p.dv, a - (float)(T)a, b - (float)(T)b, e - (float)(T)e, f - (float)(T)f);

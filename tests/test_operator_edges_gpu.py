@@ -73,6 +73,28 @@ def test_fp16_gradients_of_large_values(name, up, lone):
         A.check(got, (value, bound if more is None else bound + more.transpose(1, 2)), n)
 
 
+@pytest.mark.parametrize("Lq", [1, 50])
+def test_fp16_output_stays_within_the_values(Lq):
+    """An output is a mean of values, so finite values give finite outputs.  128 keys of score 0, then 3968 of score 1.2 u: their p = 1 + 1.2 u is
+    rounded to 1 + 2 u for the product and not in the sum, which brings the quotient to (1 + 0.77 u) times the values' 65504 -- past 65520,
+    where a conversion gives inf.  (512 heads: enough that a head's keys are not split, and its running maximum stays at the first keys')"""
+    from ic_gan_amd import ops
+    u, Lk, B, H = 2.0 ** -11, 4096, 2, 256
+    q = torch.zeros(B, Lq, H, 8, device="cuda", dtype=torch.float16)
+    q[..., 0] = 1
+    k = torch.zeros(1, Lk, 1, 8, device="cuda", dtype=torch.float16)
+    k[:, 128:, :, 0] = 1
+    for sign in (1.0, -1.0):
+        v = torch.full((1, Lk, 1, 16), 65504.0 * sign, device="cuda", dtype=torch.float16)
+        kk, vv = (t.expand(B, -1, H, -1) for t in (k, v))
+        for grad in (False, True):
+            o = ops.attention(q.detach().requires_grad_(grad), kk, vv, scale=1.2 * u).detach()
+            assert bool((o.double() * sign >= 65504 * (1 - 3 * u)).all()) and bool((o.double().abs() <= 65504).all()), o
+        v[0, 200, 0, 3] = float("inf")                           # (an infinity among the values stays one)
+        o = ops.attention(q, kk, vv, scale=1.2 * u)
+        assert not torch.isfinite(o[..., 3]).any() and torch.isfinite(o[..., :3]).all()
+
+
 # ---- keys that no query sees -----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")], ids=["nan", "inf"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=DTYPE_IDS)
