@@ -256,9 +256,16 @@ __device__ __forceinline__ int at_keys(const AttnP& p, int b) { return p.k_lens 
 // position of query 0 (clamped so that adding a query or key index cannot overflow)
 __device__ __forceinline__ int at_start(const AttnP& p, int b) { return p.q_start ? min(max(p.q_start[b], -(1 << 30)), 1 << 30) : p.Lk - p.Lq; }
 
+// A dimension of a grid holds fewer than 2^32 threads (the runtime does not refuse more, it leaves some out): rows of
+// 2^22 workgroups
+__device__ __forceinline__ int64_t at_block() { return blockIdx.x + (int64_t)gridDim.x * blockIdx.y; }
+static inline dim3 at_grid(int64_t n) { return n <= (1 << 22) ? dim3((unsigned)n) : dim3(1u << 22, (unsigned)icg_cdiv(n, 1 << 22)); }
+
 // Workgroups go to the 8 dies in turn; a run of consecutive work items per die keeps one head's keys in one die's L2.
+// (negative for a workgroup behind the last item)
 __device__ __forceinline__ int64_t at_work_item(int64_t n) {
-  const int64_t i = blockIdx.x, per = n >> 3, rest = n & 7;
+  const int64_t i = at_block(), per = n >> 3, rest = n & 7;
+  if (i >= n) return -1;
   const int64_t x = i & 7, j = i >> 3;
   return x * per + min(x, rest) + j;
 }

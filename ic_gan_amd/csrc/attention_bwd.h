@@ -13,15 +13,16 @@
 // memory order.  SCALED: the workgroups from `row_blocks` on take 128 keys of a key head each and find their largest |v_j| (finite ones: a row
 // that sees another has no finite gradient anyhow)
 template <typename T>
-__global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, float* stat, int lanes, unsigned row_blocks) {
+__global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, float* stat, int lanes, int64_t row_blocks) {
   constexpr int PER = 16 / (int)sizeof(T);
-  const int64_t rows = (int64_t)p.B * p.H * p.Lq, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int64_t block = at_block(), rows = (int64_t)p.B * p.H * p.Lq, i = (block * 256 + threadIdx.x) / lanes;
   const int l = threadIdx.x & (lanes - 1);
   if constexpr (at_type<T>::SCALED) {
-    if (blockIdx.x >= row_blocks) {
+    if (block >= row_blocks) {
       __shared__ float red[4];
-      const int64_t item = blockIdx.x - row_blocks, tiles = (p.Lk + 127) / 128, bh = item / tiles;
-      const int Hk = p.H / p.G, b = (int)(bh / Hk), hk = (int)(bh - (int64_t)b * Hk), tile = (int)(item - bh * tiles), keys = at_keys(p, b);
+      const int64_t item = block - row_blocks, tiles = (p.Lk + 127) / 128, bh = item / tiles;
+      const int Hk = p.H / p.G, b = (int)(bh / Hk), hk = (int)(bh - (int64_t)b * Hk), tile = (int)(item - bh * tiles), keys = b < p.B ? at_keys(p, b) : 0;
+      if (b >= p.B) return;
       float most = 0.f;
       for (int j = 128 * tile + (int)threadIdx.x / lanes; j < min(keys, 128 * tile + 128); j += 256 / lanes) {
         float sq = 0.f;
@@ -108,6 +109,7 @@ __global__ __launch_bounds__(256, (at_dq_waves<T, DP, DVP>())) void icg_attentio
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 31, h = lane >> 5;
   int64_t item = at_work_item(p.work);
+  if (item < 0) return;
   const int split = (int)(item % p.nsplit);
   item /= p.nsplit;
   int tile = (int)(item % p.tiles);
@@ -234,6 +236,7 @@ __global__ __launch_bounds__(256, (at_dkv_shape<T, DP, DVP>::WAVES)) void icg_at
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 31, h = lane >> 5;
   int64_t item = at_work_item(p.work);
+  if (item < 0) return;
   const int split = (int)(item % p.nsplit);
   item /= p.nsplit;
   const int tile = (int)(item % p.tiles);                // (the first keys, seen by the most queries of a causal triangle, first)
@@ -429,18 +432,18 @@ int at_bwd(AttnP p, AttnP pk, float* stat, hipStream_t st) {
   while (lanes * 16 < p.dv * (int)sizeof(T)) lanes <<= 1;        // (at most 64: rows of up to 256 fp32)
   const int64_t row_blocks = icg_cdiv((int64_t)p.B * p.H * p.Lq * lanes, 256);
   const int64_t key_blocks = at_type<T>::SCALED ? (int64_t)p.B * (p.H / p.G) * icg_cdiv(p.Lk, 128) : 0;
-  hipLaunchKernelGGL((icg_attention_rowstat_kernel<T>), dim3((unsigned)(row_blocks + key_blocks)), dim3(256), 0, st, p, stat, lanes, (unsigned)row_blocks);
+  hipLaunchKernelGGL((icg_attention_rowstat_kernel<T>), at_grid(row_blocks + key_blocks), dim3(256), 0, st, p, stat, lanes, row_blocks);
   if (const int e = icg_check_launch()) return e;
 #define AT_RUN(DP, DVP)                                                                                                  \
   do {                                                                                                                   \
-    hipLaunchKernelGGL((icg_attention_dkv_kernel<T, DP, DVP>), dim3((unsigned)pk.work), dim3(256), 0, st, pk);           \
+    hipLaunchKernelGGL((icg_attention_dkv_kernel<T, DP, DVP>), at_grid(pk.work), dim3(256), 0, st, pk);           \
     if (const int e = icg_check_launch()) return e;                                                                      \
     if (pk.nsplit > 1) {                                                                                                 \
       const int64_t quads = (int64_t)p.B * p.Lk * (p.H / p.G) * ((p.d + p.dv) / 4);                                      \
       hipLaunchKernelGGL((icg_attention_join_dkv_kernel<T>), dim3((unsigned)icg_cdiv(quads, 256)), dim3(256), 0, st, pk); \
       if (const int e = icg_check_launch()) return e;                                                                    \
     }                                                                                                                    \
-    hipLaunchKernelGGL((icg_attention_dq_kernel<T, DP, DVP>), dim3((unsigned)p.work), dim3(256), 0, st, p);              \
+    hipLaunchKernelGGL((icg_attention_dq_kernel<T, DP, DVP>), at_grid(p.work), dim3(256), 0, st, p);              \
     if (p.nsplit > 1) {                                                                                                  \
       if (const int e = icg_check_launch()) return e;                                                                    \
       const int64_t quads = (int64_t)p.B * p.H * p.Lq * (p.d / 4);                                                       \

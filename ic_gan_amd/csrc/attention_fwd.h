@@ -40,6 +40,7 @@ __global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS), (at_fwd_shape<T
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 31, h = lane >> 5;
   int64_t item = at_work_item(p.work);
+  if (item < 0) return;
   const int split = (int)(item % p.nsplit);
   item /= p.nsplit;
   int tile = (int)(item % p.tiles);
@@ -273,8 +274,8 @@ template <typename T>
 int at_fwd(const AttnP& p, bool tokens, hipStream_t st) {
 #define AT_RUN(DP, DVP)                                                                                                                    \
   do {                                                                                                                                     \
-    if (tokens) hipLaunchKernelGGL((icg_attention_fwd_kernel<T, DP, DVP, true>), dim3((unsigned)p.work), dim3(at_fwd_shape<T, true>::THREADS), 0, st, p); \
-    else hipLaunchKernelGGL((icg_attention_fwd_kernel<T, DP, DVP, false>), dim3((unsigned)p.work), dim3(at_fwd_shape<T, false>::THREADS), 0, st, p);      \
+    if (tokens) hipLaunchKernelGGL((icg_attention_fwd_kernel<T, DP, DVP, true>), at_grid(p.work), dim3(at_fwd_shape<T, true>::THREADS), 0, st, p); \
+    else hipLaunchKernelGGL((icg_attention_fwd_kernel<T, DP, DVP, false>), at_grid(p.work), dim3(at_fwd_shape<T, false>::THREADS), 0, st, p);      \
   } while (0)
   AT_FOR_HEAD(p.d, p.dv, AT_RUN)
 #undef AT_RUN

@@ -165,3 +165,22 @@ def test_norm_shows_a_gain_that_is_not_finite(shape, groups, act):
     assert torch.isnan(y[:, 3]).all()
     y[:, 3] = good[:, 3]
     assert torch.equal(y, good)
+
+
+# ---- addresses and grids beyond 32 bits ------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("Lq", [1, 17])
+def test_attention_of_more_tiles_than_a_grid_of_workgroups(Lq):
+    """2^24 sequences and some: a workgroup of 256 for each would be more threads than one dimension of a grid holds (2^32).  One key each, so
+    o is the value and its gradient the sum of do (few whole numbers: exact)."""
+    from ic_gan_amd import ops
+    B = (1 << 24) + 3
+    q, k, v = (torch.ones(B, n, 1, 8, device="cuda", dtype=torch.bfloat16) for n in (Lq, 1, 1))
+    v[:, 0, 0, 1] = torch.arange(B, device="cuda").remainder(200).bfloat16()
+    v.requires_grad_()
+    o = ops.attention(q, k, v)
+    assert all(torch.equal(a, b.expand_as(a)) for a, b in zip(o.split(1 << 22), v.detach().split(1 << 22)))
+    do = (torch.arange(B, device="cuda").remainder(3) + 1).bfloat16().view(B, 1, 1, 1).expand(B, Lq, 1, 8)
+    (dv,) = torch.autograd.grad(o, v, do)
+    assert torch.equal(dv, (do[:, :1] * Lq))
