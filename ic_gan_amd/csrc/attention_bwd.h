@@ -244,7 +244,8 @@ __global__ __launch_bounds__(256, (at_dkv_shape<T, DP, DVP>::WAVES)) void icg_at
   const int Hk = p.H / p.G, b = (int)(bh / Hk), hk = (int)(bh - (int64_t)b * Hk);
   const int j = 128 * tile + 32 * wv + m;
   const int keys = at_keys(p, b), start = at_start(p, b);
-  const bool valid = j < keys;
+  // a key that some query sees; the others are read as zeros (NaN or infinity there would meet the zero rows that fill the last query tile)
+  const bool valid = j < keys && (!p.causal || j < start + p.Lq);
   const int64_t rows = (int64_t)p.B * p.H * p.Lq, row_b = ((int64_t)b * p.H + hk * p.G) * p.Lq;
 
   frag kf[DP / X::KSTEP], vf[DVP / X::KSTEP];
@@ -327,8 +328,7 @@ __global__ __launch_bounds__(256, (at_dkv_shape<T, DP, DVP>::WAVES)) void icg_at
       for (int t = 0; t < DVP / X::KSTEP; ++t) dp = X::mma(gr.row_frag(gt, 32 * u, t), vf[t], dp);
       const int first = valid ? (p.causal ? j - start : -(1 << 30)) : 0x7fffffff;       // the first query that sees this lane's key
       const int r0 = (i0 + t0) * QT + 32 * u;
-      // (rows from Lq on are zeros: with a key of NaN or infinity, which may lie where no query sees it, even they would leave NaN)
-      const bool edge = __any(r0 < first) || r0 + 32 > p.Lq;
+      const bool edge = __any(r0 < first);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const at_f4 l4 = *reinterpret_cast<const at_f4*>(stat + 32 * u + 8 * g + 4 * h), d4 = *reinterpret_cast<const at_f4*>(stat + QT + 32 * u + 8 * g + 4 * h);
@@ -342,8 +342,7 @@ __global__ __launch_bounds__(256, (at_dkv_shape<T, DP, DVP>::WAVES)) void icg_at
       if (edge) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int row = r0 + at_row_of(i, h);
-          const bool off = row < first || row >= p.Lq;
+          const bool off = r0 + at_row_of(i, h) < first;
           s[i] = off ? 0.f : s[i];
           dp[i] = off ? 0.f : dp[i];
         }
