@@ -229,7 +229,8 @@ __global__ __launch_bounds__(64) void icg_embedding_bwd_piece_kernel(EmbP p) {
 // a wave per column tile of a row of the table: the longest piece of work is a tile of EMB_CHUNK entries, or of one sum per EMB_CHUNK entries
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void icg_embedding_bwd_row_kernel(EmbP p, int tiles) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), v = w / tiles, c = ((w - v * tiles) * 64 + (threadIdx.x & 63)) * VEC;
+  const int64_t w = (blockIdx.x + (int64_t)gridDim.x * blockIdx.y) * 4 + (threadIdx.x >> 6), v = w / tiles;
+  const int64_t c = ((w - v * tiles) * 64 + (threadIdx.x & 63)) * VEC;
   if (v >= p.V || c >= p.D) return;
   const int b = p.start[v], e = p.start[v + 1];
   float a[VEC];
@@ -260,8 +261,11 @@ __global__ __launch_bounds__(256) void icg_embedding_bwd_row_kernel(EmbP p, int 
   }
   em_write<T, VEC>(a, p, v, c);
 }
-
 namespace {
+
+// A dimension of a grid holds fewer than 2^32 threads, and the runtime does not refuse more, it leaves some out.  The lookup and the gradient of
+// few tokens stride over what a capped grid leaves; the rows of the sorted gradient (a loop around them costs 4 %) take a second dimension.
+unsigned em_blocks(int64_t n) { return (unsigned)(n < ICG_GRID_CAP ? n : ICG_GRID_CAP); }
 
 // (column tiles of 64 elements at the narrowest are a grid's second dimension: at most 32768 of them)
 bool em_shape_ok(int64_t n, int64_t V, int64_t D, int dtype) {
@@ -271,26 +275,23 @@ size_t em_align(size_t x) { return (x + 15) / 16 * 16; }
 
 template <typename T, int VEC>
 int em_fwd(const EmbP& p, hipStream_t st) {
-  const int64_t blocks = icg_cdiv(p.n * (p.D / VEC), 256);
-  const int64_t cap = ICG_GRID_CAP;
-  hipLaunchKernelGGL((icg_embedding_fwd_kernel<T, VEC>), dim3((unsigned)(blocks < cap ? blocks : cap)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((icg_embedding_fwd_kernel<T, VEC>), dim3(em_blocks(icg_cdiv(p.n * (p.D / VEC), 256))), dim3(256), 0, st, p);
   return icg_check_launch();
 }
 
 template <typename T, int VEC>
 int em_bwd(const EmbP& p, hipStream_t st) {
-  const unsigned rows = (unsigned)icg_cdiv(p.V, 4);
   if (p.n <= EMB_FEW) {
-    hipLaunchKernelGGL((icg_embedding_bwd_few_kernel<T, VEC>), dim3(rows), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((icg_embedding_bwd_few_kernel<T, VEC>), dim3(em_blocks(icg_cdiv(p.V, 4))), dim3(256), 0, st, p);
     return icg_check_launch();
   }
   hipLaunchKernelGGL(icg_embedding_sort_kernel, dim3((unsigned)icg_cdiv(p.V, p.run)), dim3(64 * EMB_WAVES), 0, st, p);
   if (const int e = icg_check_launch()) return e;
   hipLaunchKernelGGL((icg_embedding_bwd_piece_kernel<T, VEC>), dim3((unsigned)icg_cdiv(p.n, EMB_CHUNK), (unsigned)icg_cdiv(p.D, 64 * VEC), 2), dim3(64), 0, st, p);
   if (const int e = icg_check_launch()) return e;
-  const int64_t tiles = icg_cdiv(p.D, 64 * VEC), blocks = icg_cdiv(p.V * tiles, 4);
-  ICG_REQUIRE(blocks < 0x7fffffffLL);
-  hipLaunchKernelGGL((icg_embedding_bwd_row_kernel<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, p, (int)tiles);
+  const int64_t tiles = icg_cdiv(p.D, 64 * VEC), blocks = icg_cdiv(p.V * tiles, 4), wide = blocks < (1 << 22) ? blocks : 1 << 22;
+  ICG_REQUIRE(icg_cdiv(blocks, wide) < 65536);
+  hipLaunchKernelGGL((icg_embedding_bwd_row_kernel<T, VEC>), dim3((unsigned)wide, (unsigned)icg_cdiv(blocks, wide)), dim3(256), 0, st, p, (int)tiles);
   return icg_check_launch();
 }
 

@@ -170,6 +170,51 @@ def test_norm_shows_a_gain_that_is_not_finite(shape, groups, act):
 # ---- addresses and grids beyond 32 bits ------------------------------------------------------------------------------------------------
 
 
+@pytest.mark.parametrize("n", [20, 1500], ids=["few", "sorted"])
+def test_embedding_table_beyond_two_to_the_31_elements(n):
+    from ic_gan_amd import ops
+    V, D = (1 << 22) + 3, 520
+    w = torch.zeros(V, D, dtype=torch.bfloat16, device="cuda")
+    idx = torch.cat([torch.arange(V - n // 2, V), torch.arange(n - n // 2)]).cuda()
+    assert V * D > 2 ** 31 and (V - n // 2) * D > 2 ** 31
+    rows = torch.randn(n, D, device="cuda").bfloat16()
+    w[idx] = rows
+    w.requires_grad_()
+    out = ops.embedding(idx, w)
+    assert torch.equal(out, rows)
+    (dw,) = torch.autograd.grad(out, w, rows.flip(0))
+    assert torch.equal(dw[idx], rows.flip(0))                    # (each token once: copies)
+    dw[idx] = 0
+    assert not any(bool(part.any()) for part in dw.split(1 << 20))
+
+
+def test_embedding_output_beyond_two_to_the_31_elements():
+    from ic_gan_amd import ops
+    V, D, n = 11, 520, (1 << 22) + 5
+    assert n * D > 2 ** 31
+    w = torch.randn(V, D, device="cuda").bfloat16().requires_grad_()
+    idx = torch.randint(0, V, (n,), device="cuda")
+    out = ops.embedding(idx, w)
+    assert torch.equal(out[-1000:], w.detach()[idx[-1000:]]) and torch.equal(out[:1000], w.detach()[idx[:1000]])
+    dout = torch.zeros_like(out)
+    dout[-100:] = torch.randint(-8, 9, (100, D), device="cuda").bfloat16()
+    (dw,) = torch.autograd.grad(out, w, dout)
+    want = torch.zeros(V, D, device="cuda").index_add_(0, idx[-100:], dout[-100:].float())       # (whole numbers below 2^11: exact)
+    assert torch.equal(dw.float(), want.bfloat16().float())
+
+
+@pytest.mark.parametrize("n", [9, 1030], ids=["few", "sorted"])
+def test_embedding_gradient_of_more_rows_than_a_grid_of_waves(n):
+    """2^26 rows and some: a wave for each would be more threads than one dimension of a grid holds (2^32)"""
+    from ic_gan_amd import ops
+    V, D = (1 << 26) + 7, 3
+    w = torch.zeros(V, D, device="cuda", requires_grad=True)
+    idx = torch.cat([torch.arange(V - n + 3, V), torch.tensor([0, 5, 5])]).cuda()
+    (dw,) = torch.autograd.grad(ops.embedding(idx, w), w, torch.ones(n, D, device="cuda"))
+    assert bool((dw[V - n + 3:] == 1).all()) and bool((dw[0] == 1).all()) and bool((dw[5] == 2).all())
+    assert float(dw.sum(dtype=torch.float64)) == n * D
+
+
 @pytest.mark.parametrize("Lq", [1, 17])
 def test_attention_of_more_tiles_than_a_grid_of_workgroups(Lq):
     """2^24 sequences and some: a workgroup of 256 for each would be more threads than one dimension of a grid holds (2^32).  One key each, so
