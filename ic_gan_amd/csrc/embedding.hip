@@ -6,7 +6,8 @@
 // atomics and without a general sort: a workgroup owns a run of tokens, scans the whole list (it stays in L2), and learns in one
 // sweep how often each of its tokens occurs in each wave's share of the list and how many entries belong to smaller tokens, which is where its
 // part of the sorted list begins; a second sweep puts the positions in place.  Tokens that occur often are summed in pieces of
-// EMB_CHUNK list entries, so that the longest row of work is bounded however skewed the tokens are.
+// EMB_CHUNK list entries first.  What one wave does in turn still grows with its token: n / EMB_CHUNK sums of pieces for a token that fills
+// the list, and up to EMB_FEW entries, 8 loads at a time, where the list is short and not sorted.
 // Measured, 50000 x 2048 bf16, 16384 skewed tokens: lookup 25 us (5.4 TB/s), order 17 us (the busiest run's entries, one after the other), pieces
 // 13 us, rows 69 us (4.0 TB/s); 1000 x 128 fp32, 64 tokens: 3 us each way.
 #include "icg_common.h"
@@ -78,9 +79,10 @@ __device__ __forceinline__ void em_write(const float (&a)[VEC], const EmbP& p, i
   em_store<T, VEC>(reinterpret_cast<T*>(p.dw) + v * p.D + c, o);
 }
 
-// few tokens: the list in LDS, a wave per row of the table finds its entries by ballot
+// few tokens: the list in LDS, a wave per column tile of a row of the table finds its entries by ballot and adds them in order, up to 8 loads in
+// flight
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void icg_embedding_bwd_few_kernel(EmbP p) {
+__global__ __launch_bounds__(256) void icg_embedding_bwd_few_kernel(EmbP p, int tiles) {
   __shared__ int list[EMB_FEW];
   const int n = (int)p.n;
   for (int i = threadIdx.x; i < n; i += 256) {
@@ -89,22 +91,32 @@ __global__ __launch_bounds__(256) void icg_embedding_bwd_few_kernel(EmbP p) {
   }
   __syncthreads();
   const int lane = threadIdx.x & 63;
-  for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < p.V; v += (int64_t)gridDim.x * 4)
-    for (int64_t c0 = 0; c0 < p.D; c0 += 64 * VEC) {
-      const int64_t c = c0 + lane * VEC;
-      float a[VEC];
+  for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); w < p.V * tiles; w += (int64_t)gridDim.x * 4) {
+    const int64_t v = w / tiles, c = ((w - v * tiles) * 64 + lane) * VEC;
+    float a[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) a[j] = 0.f;
-      for (int i0 = 0; i0 < n; i0 += 64) {
-        unsigned long long hit = __ballot(i0 + lane < n && list[min(i0 + lane, n - 1)] == (int)v);
-        while (hit) {
-          const int i = i0 + __builtin_ctzll(hit);
-          hit &= hit - 1;
-          if (c < p.D) em_add<T, VEC>(a, p, i, c);
-        }
+    for (int j = 0; j < VEC; ++j) a[j] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 64) {
+      unsigned long long hit = __ballot(i0 + lane < n && list[min(i0 + lane, n - 1)] == (int)v);
+      while (hit) {
+        em_vec<T, VEC> x[8];
+        int m = 0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (hit) {
+            const int i = i0 + __builtin_ctzll(hit);
+            hit &= hit - 1, ++m;
+            if (c < p.D) x[q] = em_load<T, VEC>(reinterpret_cast<const T*>(p.dout) + (int64_t)i * p.D + c);
+          }
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < m)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) a[j] += (float)x[q].e[j];
       }
-      if (c < p.D) em_write<T, VEC>(a, p, v, c);
     }
+    if (c < p.D) em_write<T, VEC>(a, p, v, c);
+  }
 }
 
 // ---- the positions in the order of their tokens
@@ -281,15 +293,15 @@ int em_fwd(const EmbP& p, hipStream_t st) {
 
 template <typename T, int VEC>
 int em_bwd(const EmbP& p, hipStream_t st) {
+  const int64_t tiles = icg_cdiv(p.D, 64 * VEC), blocks = icg_cdiv(p.V * tiles, 4), wide = blocks < (1 << 22) ? blocks : 1 << 22;
   if (p.n <= EMB_FEW) {
-    hipLaunchKernelGGL((icg_embedding_bwd_few_kernel<T, VEC>), dim3(em_blocks(icg_cdiv(p.V, 4))), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((icg_embedding_bwd_few_kernel<T, VEC>), dim3(em_blocks(blocks)), dim3(256), 0, st, p, (int)tiles);
     return icg_check_launch();
   }
   hipLaunchKernelGGL(icg_embedding_sort_kernel, dim3((unsigned)icg_cdiv(p.V, p.run)), dim3(64 * EMB_WAVES), 0, st, p);
   if (const int e = icg_check_launch()) return e;
   hipLaunchKernelGGL((icg_embedding_bwd_piece_kernel<T, VEC>), dim3((unsigned)icg_cdiv(p.n, EMB_CHUNK), (unsigned)icg_cdiv(p.D, 64 * VEC), 2), dim3(64), 0, st, p);
   if (const int e = icg_check_launch()) return e;
-  const int64_t tiles = icg_cdiv(p.D, 64 * VEC), blocks = icg_cdiv(p.V * tiles, 4), wide = blocks < (1 << 22) ? blocks : 1 << 22;
   ICG_REQUIRE(icg_cdiv(blocks, wide) < 65536);
   hipLaunchKernelGGL((icg_embedding_bwd_row_kernel<T, VEC>), dim3((unsigned)wide, (unsigned)icg_cdiv(blocks, wide)), dim3(256), 0, st, p, (int)tiles);
   return icg_check_launch();
