@@ -491,6 +491,24 @@ GnP gn_params(const GnPlan& pl, int B, int64_t HW, int C, int G, int per_sample,
   return p;
 }
 
+int gn_width(const GnPlan& pl, int dtype) { return !pl.vec ? 1 : dtype == 0 ? 4 : 8; }
+// A dimension of a grid holds fewer than 2^32 threads (the runtime does not refuse more, it leaves some out)
+bool gn_grids_ok(const GnPlan& pl, int B, int64_t HW, int G, bool bwd, int vec) {
+  const int64_t most = 1LL << 32;
+  if (pl.slab) return (int64_t)B * pl.ncol * pl.threads < most;
+  return pl.ncol < 65536 && (int64_t)B * G * 256 < most && (int64_t)pl.nchunks * 256 < most &&
+         icg_cdiv(HW, pl.ny * gn_apply_rows(vec, bwd)) * 256 < most;
+}
+// both directions, with 16-byte columns and without
+bool gn_applies(int B, int64_t HW, int C, int G, int dtype) {
+  if (!gn_shape_ok(B, HW, C, G, dtype)) return false;
+  for (int i = 0; i < 4; ++i) {
+    const GnPlan pl = gn_plan(B, HW, C, G, dtype, i & 1, i >> 1);
+    if (!gn_grids_ok(pl, B, HW, G, i >> 1, gn_width(pl, dtype))) return false;
+  }
+  return true;
+}
+
 template <typename T, int VEC, bool BWD>
 int gn_run(const GnPlan& pl, const GnP& p, hipStream_t st) {
   if (pl.slab) {
@@ -521,6 +539,8 @@ int gn_dispatch(const GnPlan& pl, const GnP& p, int dtype, hipStream_t st) {
 
 }  // namespace
 
+extern "C" int icg_groupnorm_applies(int B, int64_t HW, int C, int G, int dtype) { return gn_applies(B, HW, C, G, dtype) ? 1 : 0; }
+
 extern "C" size_t icg_groupnorm_fwd_workspace_bytes(int B, int64_t HW, int C, int G, int dtype) {
   return gn_shape_ok(B, HW, C, G, dtype) ? gn_part_bytes(B, HW, C, G, dtype, false) : 0;
 }
@@ -531,7 +551,7 @@ extern "C" int icg_groupnorm_act_fwd(const void* x, const float* gain, const flo
   ICG_REQUIRE(x && y && mean && rstd && gn_shape_ok(B, HW, C, G, dtype) && act >= 0 && act <= 2 && eps >= 0.f && eps < INFINITY);
   const bool vec = ((uintptr_t)x % 16) == 0 && ((uintptr_t)y % 16) == 0;
   const GnPlan pl = gn_plan(B, HW, C, G, dtype, vec, false);
-  ICG_REQUIRE((int64_t)B * pl.ncol < 0x7fffffffL && pl.ncol < 65536);
+  ICG_REQUIRE(gn_grids_ok(pl, B, HW, G, false, gn_width(pl, dtype)));
   GnP p = gn_params(pl, B, HW, C, G, per_sample, gain_offset, eps, act);
   p.x = x, p.gain = gain, p.bias = bias, p.y = y, p.mean = mean, p.rstd = rstd;
   if (!pl.slab) {
@@ -554,7 +574,7 @@ extern "C" int icg_groupnorm_act_bwd(const void* x, const void* dy, const float*
   ICG_REQUIRE(workspace && ((uintptr_t)workspace % 16) == 0);
   const bool vec = ((uintptr_t)x % 16) == 0 && ((uintptr_t)dy % 16) == 0 && ((uintptr_t)dx % 16) == 0;
   const GnPlan pl = gn_plan(B, HW, C, G, dtype, vec, true);
-  ICG_REQUIRE((int64_t)B * pl.ncol < 0x7fffffffL && pl.ncol < 65536);
+  ICG_REQUIRE(gn_grids_ok(pl, B, HW, G, true, gn_width(pl, dtype)));
   GnP p = gn_params(pl, B, HW, C, G, per_sample, gain_offset, eps, act);
   p.x = x, p.dy = dy, p.gain = gain, p.bias = bias, p.dx = dx, p.mean = const_cast<float*>(mean), p.rstd = const_cast<float*>(rstd);
   p.part = (float*)workspace;

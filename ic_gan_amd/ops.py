@@ -1555,6 +1555,8 @@ def group_norm_act(x, groups, gain=None, bias=None, *, eps=1e-5, act="none", gai
             raise ValueError("group_norm_act: %s is on %s, x on %s" % (name, t.device, x.device))
     if gain is not None and bias is not None and gain.shape != bias.shape:
         raise ValueError("group_norm_act: gain %s and bias %s differ in shape" % (tuple(gain.shape), tuple(bias.shape)))
+    if x.numel() and not _host_plan("icg_groupnorm_applies", B, x.shape[2] * x.shape[3], C, groups, _DTYPE_CODES[x.dtype]):
+        raise ValueError("group_norm_act: not served: x %s (fewer than 2^16 samples, 2^30 pixels and 2^20 channels)" % (tuple(x.shape),))
     _require_gpu(x)
     gain, bias = (t if t is None else t.float().contiguous() for t in (gain, bias))
     return GroupNormActFn.apply(x, gain, bias, groups, float(gain_offset), float(eps), _ACTIVATIONS[act])

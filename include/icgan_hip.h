@@ -812,7 +812,9 @@ int icg_attention_bwd(const void* q, const void* k, const void* v, const void* o
  *   y = act(xh (g0 + gain) + bias),  xh = (x - m) / sqrt(v + eps),  m, v over HW and the C / G channels of a group, per sample
  * x, y, dy, dx [B][HW][C] of dtype 0 / 1 / 2 = fp32 / fp16 / bf16; gain, bias (NULL: 1 and 0), dgain, dbias fp32 [C], or [B][C] with per_sample;
  * act 0 none, 1 ReLU, 2 SiLU.  mean, rstd [B][G] fp32 leave the forward and enter the gradient, which forms act' again from x.  dgain and
- * dbias may both be NULL.  One launch where a group's slab fits a workgroup's registers, three (x read twice) elsewhere. */
+ * dbias may both be NULL.  One launch where a group's slab fits a workgroup's registers, three (x read twice) elsewhere.  `_applies`: fewer than
+ * 2^16 samples, 2^30 pixels and 2^20 channels, and launches within the runtime's limits (both directions); other sizes are refused. */
+int icg_groupnorm_applies(int B, int64_t HW, int C, int G, int dtype);
 size_t icg_groupnorm_fwd_workspace_bytes(int B, int64_t HW, int C, int G, int dtype);
 int icg_groupnorm_act_fwd(const void* x, const float* gain, const float* bias, void* y, float* mean, float* rstd, int B, int64_t HW, int C, int G,
                           int per_sample, float gain_offset, float eps, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);

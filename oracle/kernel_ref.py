@@ -1579,6 +1579,10 @@ def icg_attention_bwd(q, k, v, o, o_low, dout, lse, k_lens, q_start, dq, dk, dv_
     dv_out.copy_(shared(p.transpose(-1, -2) @ dO))
 
 
+def icg_groupnorm_applies(B, HW, C, G, dtype):
+    return int(0 < B < 1 << 16 and 0 < HW < 1 << 30 and 0 < C < 1 << 20 and G > 0 and C % G == 0 and dtype in (0, 1, 2))
+
+
 def icg_groupnorm_fwd_workspace_bytes(*a):
     return 0
 

@@ -49,3 +49,28 @@ def test_a_gradient_with_a_tangent_is_refused(name, monkeypatch):
             assert torch.equal(a, b)
         with pytest.raises(NotImplementedError):
             torch.autograd.grad(y, ins, forward_ad.make_dual(torch.ones_like(y), torch.randn_like(y)))
+
+
+def test_norm_sizes_are_refused_with_the_arguments():
+    """a ValueError like every other refusal, before anything is launched"""
+    from ic_gan_amd import ops
+    for shape, groups in (((65536, 4, 1, 1), 2), ((1, 4, 1 << 15, 1 << 15), 2), ((1, 1 << 20, 1, 1), 1), ((60000, 1024, 1024, 1024), 1024)):
+        with pytest.raises(ValueError, match="not served"):
+            ops.group_norm_act(torch.empty(shape, device="meta"), groups)
+    for shape in ((0, 8, 4, 4), (65535, 1024, 1, 1)):
+        with pytest.raises(RuntimeError, match="AMD GPU only"):
+            ops.group_norm_act(torch.empty(shape, device="meta"), 2)
+
+
+def test_norm_entry_points_refuse_grids_beyond_the_launch_limit():
+    import ctypes
+    from ic_gan_amd import _lib
+    lib = _lib.lib()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 15) & ~15
+    fwd = lambda B, HW, C, G: lib.icg_groupnorm_act_fwd(p, None, None, p, p, p, B, HW, C, G, 0, 0.0, 1e-5, 0, 0, p, 1 << 60, None)
+    bwd = lambda B, HW, C, G: lib.icg_groupnorm_act_bwd(p, p, None, None, p, p, p, None, None, B, HW, C, G, 0, 0.0, 1e-5, 0, 0, p, 1 << 60, None)
+    for B, HW, C, G in ((65536, 1, 4, 2), (1, 1 << 30, 4, 2), (60000, 1 << 20, 1024, 1024), (1, (1 << 30) - 1, 4097, 1)):
+        assert lib.icg_groupnorm_applies(B, HW, C, G, 0) == 0 and fwd(B, HW, C, G) == -1 and bwd(B, HW, C, G) == -1
+    assert lib.icg_groupnorm_applies(64, 65536, 96, 16, 0) == 1 and lib.icg_groupnorm_applies(1, 1, 1, 1, 2) == 1
+    assert lib.icg_groupnorm_applies(2, 4, 8, 3, 0) == 0 and lib.icg_groupnorm_applies(2, 4, 8, 2, 3) == 0

@@ -168,6 +168,22 @@ def test_norm_shows_a_gain_that_is_not_finite(shape, groups, act):
 
 
 # ---- addresses and grids beyond 32 bits ------------------------------------------------------------------------------------------------
+def test_norm_beyond_two_to_the_31_elements():
+    """65 samples of 33.5 million elements: the last one begins at element 2^31.  Values and gradients are those of the sample alone, but for
+    the chunks that its sums are formed in (equal up to fp32 rounding, so outputs are within one step of bf16)."""
+    from ic_gan_amd import ops
+    shape = (65, 64, 512, 1024)
+    assert (shape[0] - 1) * 64 * 512 * 1024 >= 2 ** 31
+    x, dy = (torch.empty(shape, dtype=torch.bfloat16, device="cuda", memory_format=torch.channels_last).normal_() for _ in range(2))
+    x.requires_grad_()
+    y = ops.group_norm_act(x, 8, act="silu")
+    (dx,) = torch.autograd.grad(y, x, dy)
+    last = x.detach()[-1:].clone().requires_grad_()
+    z = ops.group_norm_act(last, 8, act="silu")
+    (dz,) = torch.autograd.grad(z, last, dy[-1:])
+    for a, b in ((y[-1:], z), (dx[-1:], dz)):
+        a, b = a.detach().float(), b.detach().float()
+        assert float(b.abs().max()) > 1 and float(((a - b).abs() / (b.abs() + 1e-2)).max()) <= 2 ** -7
 
 
 @pytest.mark.parametrize("n", [20, 1500], ids=["few", "sorted"])
