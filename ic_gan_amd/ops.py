@@ -1533,7 +1533,7 @@ def group_norm_act(x, groups, gain=None, bias=None, *, eps=1e-5, act="none", gai
     """act(group_norm(x) * (gain_offset + gain) + bias) in the layout of x [B, C, H, W] (channels last; another layout is converted).
 
     x: fp32, fp16 or bf16; statistics and arithmetic in fp32, one rounding.  groups divides C.  gain, bias: [C], or [B, C] for a
-    conditional norm (both of one shape; None: 1 and 0).  act: "none", "relu" or "silu".  Differentiable once in x, gain and bias; nothing but
+    conditional norm (both of one shape, fp32, fp16 or bf16; None: 1 and 0).  act: "none", "relu" or "silu".  Differentiable once in x, gain and bias; nothing but
     x and the groups' mean and 1 / deviation is kept for the gradient."""
     if not isinstance(x, torch.Tensor) or x.dim() != 4:
         raise ValueError("group_norm_act: x must be a 4-D activation [batch, channel, height, width]")
@@ -1549,8 +1549,8 @@ def group_norm_act(x, groups, gain=None, bias=None, *, eps=1e-5, act="none", gai
     for name, t in (("gain", gain), ("bias", bias)):
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or tuple(t.shape) not in ((C,), (B, C)) or not t.is_floating_point():
-            raise ValueError("group_norm_act: %s must be a floating-point tensor of shape [%d] or [%d, %d]" % (name, C, B, C))
+        if not isinstance(t, torch.Tensor) or tuple(t.shape) not in ((C,), (B, C)) or t.dtype not in _DTYPE_CODES:
+            raise ValueError("group_norm_act: %s must be an fp32, fp16 or bf16 tensor of shape [%d] or [%d, %d]" % (name, C, B, C))
         if t.device != x.device:
             raise ValueError("group_norm_act: %s is on %s, x on %s" % (name, t.device, x.device))
     if gain is not None and bias is not None and gain.shape != bias.shape:

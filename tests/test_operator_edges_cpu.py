@@ -62,6 +62,14 @@ def test_norm_sizes_are_refused_with_the_arguments():
             ops.group_norm_act(torch.empty(shape, device="meta"), 2)
 
 
+def test_a_64_bit_gain_is_refused():
+    from ic_gan_amd import ops
+    x, one = torch.zeros(2, 8, 3, 3), torch.ones(8)
+    for gain, bias, match in ((one.double(), one, "gain must be"), (one, one.double(), "bias must be"), (None, one.double(), "bias must be")):
+        with pytest.raises(ValueError, match=match):
+            ops.group_norm_act(x, 2, gain, bias)
+
+
 def test_norm_entry_points_refuse_grids_beyond_the_launch_limit():
     import ctypes
     from ic_gan_amd import _lib
