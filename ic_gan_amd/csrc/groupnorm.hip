@@ -435,6 +435,9 @@ bool gn_shape_ok(int B, int64_t HW, int C, int G, int dtype) {
   return B > 0 && B < 65536 && HW > 0 && HW < (1LL << 30) && C > 0 && C < (1 << 20) && G > 0 && C % G == 0 && dtype >= 0 && dtype <= 2 && (int64_t)B * G < 0x7fffffffL;
 }
 
+// whether the one-pass kernel has a form of 1024 threads (128 registers each: too few for 8 rows of x and dy in 16 bits)
+constexpr bool gn_wide(int vec, bool bwd) { return !(bwd && vec == 8); }
+
 GnPlan gn_plan(int B, int64_t HW, int C, int G, int dtype, bool vec, bool bwd) {
   GnPlan pl = {};
   const int per = dtype == 0 ? 4 : 8, v = vec && C % per == 0 ? per : 1, Cg = C / G;
@@ -444,8 +447,7 @@ GnPlan gn_plan(int B, int64_t HW, int C, int G, int dtype, bool vec, bool bwd) {
   int gs = 1;
   while (gs <= G && (G % gs != 0 || (gs * Cg) % v != 0)) ++gs;
   auto fits = [&](int set, int threads) { const int cc = set * Cg / v; return cc <= threads && HW <= (int64_t)(threads / cc) * GN_R; };
-  const bool wide = !(bwd && v == 8);                      // (1024 threads have 128 registers each: too few for 8 rows of x and dy in 16 bits)
-  if (gs <= G && (fits(gs, 256) || (wide && fits(gs, 1024)))) {
+  if (gs <= G && (fits(gs, 256) || (gn_wide(v, bwd) && fits(gs, 1024)))) {
     pl.slab = true;
     while (G % (2 * gs) == 0 && fits(2 * gs, 256) && (int64_t)B * (G / (2 * gs)) >= 512) gs *= 2;
     pl.threads = fits(gs, 256) ? 256 : 1024;
@@ -513,8 +515,13 @@ template <typename T, int VEC, bool BWD>
 int gn_run(const GnPlan& pl, const GnP& p, hipStream_t st) {
   if (pl.slab) {
     const dim3 grid((unsigned)((int64_t)p.B * p.ncol));
-    if (pl.threads == 256) hipLaunchKernelGGL((icg_groupnorm_slab_kernel<T, VEC, 256, BWD>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((icg_groupnorm_slab_kernel<T, VEC, 1024, BWD>), grid, dim3(1024), 0, st, p);
+    if constexpr (gn_wide(VEC, BWD)) {
+      if (pl.threads == 1024) {
+        hipLaunchKernelGGL((icg_groupnorm_slab_kernel<T, VEC, 1024, BWD>), grid, dim3(1024), 0, st, p);
+        return icg_check_launch();
+      }
+    }
+    hipLaunchKernelGGL((icg_groupnorm_slab_kernel<T, VEC, 256, BWD>), grid, dim3(256), 0, st, p);
     return icg_check_launch();
   }
   const dim3 grid((unsigned)pl.nchunks, (unsigned)pl.ncol, (unsigned)p.B);
