@@ -82,3 +82,39 @@ def test_norm_entry_points_refuse_grids_beyond_the_launch_limit():
         assert lib.icg_groupnorm_applies(B, HW, C, G, 0) == 0 and fwd(B, HW, C, G) == -1 and bwd(B, HW, C, G) == -1
     assert lib.icg_groupnorm_applies(64, 65536, 96, 16, 0) == 1 and lib.icg_groupnorm_applies(1, 1, 1, 1, 2) == 1
     assert lib.icg_groupnorm_applies(2, 4, 8, 3, 0) == 0 and lib.icg_groupnorm_applies(2, 4, 8, 2, 3) == 0
+
+
+class _On(torch.Tensor):
+    """a host tensor that says it is on a device"""
+    device_index = 0
+
+    def get_device(self):
+        return self.device_index
+
+
+@pytest.mark.parametrize("current,tensor", [(0, 0), (0, 3), (2, 1)])
+def test_a_kernel_goes_to_the_device_and_stream_of_its_tensors(current, tensor, monkeypatch):
+    from ic_gan_amd import _lib
+    state, seen = {"device": current}, []
+
+    class device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, state["device"] = state["device"], self.index
+
+        def __exit__(self, *a):
+            state["device"] = self.before
+    t = torch.zeros(4).as_subclass(_On)
+    t.device_index = tensor
+    monkeypatch.setattr(_lib, "_raw_stream", lambda d: 1000 + d)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: state["device"], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setitem(_lib._bound, "icg_pretended", lambda *a: seen.append((state["device"],) + a) or 0)
+    _lib.call("icg_pretended", None, 7, t, 2.5)
+    assert seen == [(tensor, None, 7, t.data_ptr(), 2.5, 1000 + tensor)] and state["device"] == current
+    monkeypatch.setitem(_lib._bound, "icg_pretended", lambda *a: -1)
+    with pytest.raises(RuntimeError, match="icg_pretended failed"):
+        _lib.call("icg_pretended", t)
+    assert state["device"] == current

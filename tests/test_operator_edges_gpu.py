@@ -248,6 +248,27 @@ def test_attention_of_more_tiles_than_a_grid_of_workgroups(Lq):
 
 
 # ---- the spectral-norm embedding's gradient, its correction term included --------------------------------------------------------------
+def test_gradient_of_a_large_spectral_norm_table():
+    """layers.SNEmbedding with more labels than the one-hot product takes.  With the vectors of its own power-iteration step, u, v and
+    sigma = v W^T u^T, the gradient is (raw - <raw, W> / sigma u^T v) / sigma.  dout is the output itself, so that the correction is a third of
+    the raw gradient's norm.  The sums of 640 000 products in 32 bits are off by about sqrt(n) w = 5e-5 of their terms: 2e-4 of the norm."""
+    from ic_gan_amd import layers
+    torch.manual_seed(0)
+    m = layers.SNEmbedding(40000, 16).cuda().train()
+    y = torch.randint(0, 300, (2000,), device="cuda")
+    u0, w = m.u0.detach().double().clone(), m.weight.detach().double()
+    out = m(y)
+    d = out.detach().clone()
+    out.backward(d)
+    v = torch.nn.functional.normalize(u0 @ w, dim=1)
+    u = torch.nn.functional.normalize(v @ w.t(), dim=1)
+    sigma = float(v @ w.t() @ u.t())
+    assert float((m.u0.double() - u).norm()) < 1e-5
+    raw = torch.zeros(40000, 16, dtype=torch.float64, device="cuda").index_add_(0, y, d.double())
+    correction = float((raw * w).sum()) / sigma * (u.t() @ v)
+    want = (raw - correction) / sigma
+    assert float(correction.norm()) > 0.2 * float(raw.norm())
+    assert float((m.weight.grad.double() - want).norm()) <= 2e-4 * float(want.norm())
 
 
 @pytest.mark.parametrize("V,D,n,kind", [(70000, 128, 1024, "same"), (10, 4095, 1024, "uniform"), (5, 4096, 1024, "same")])
