@@ -4,13 +4,14 @@
 #pragma once
 #include "attention.h"
 
-// Measured, 2 x 4096 causal, 16 heads of 128 over 4 key heads, bf16: row sums 23 us, dk and dv 373 us (740 TFLOP/s), their join 14 us, dq 270 us
-// (765 TFLOP/s); 64 x 4096 queries, 1024 keys, 24 / 96 elements, fp32: 39, 1130 (114), -, 705 us (109 TFLOP/s).  Bound like the forward kernel by
-// products plus vector instructions of a SIMD, one after the other.
+// Measured (kernel trace), 2 x 4096 causal, 16 heads of 128 over 4 key heads, bf16: row sums 23 us, dk and dv 375 us (733 TFLOP/s), their join
+// 14 us, dq 272 us (758 TFLOP/s); 64 x 4096 queries, 1024 keys, 24 / 96 elements, fp32: 41, 1088 (118), -, 691 us (112 TFLOP/s); 6 x 777 queries, up to
+// 1033 keys, 5 heads of 80, fp16: 10 (5 of them for the largest |v|), 50, -, 31 us.  Bound like the forward kernel: products and vector
+// instructions of a SIMD add up to 0.93 of its cycles in fp32, 0.86 in the bf16 dq; dk and dv in bf16 have one wave a SIMD (0.73).
 
 // D_i = do_i . o_i, |do_i| and the exponent's offset; o_i as it was before its rounding to 16 bits where the forward kept the rest (dp - D
-// cancels: with the rounded o, a row of few keys had twice the error of its products' operands); `lanes` lanes (the power of two that covers a row's 16-byte chunks) to a row, rows in
-// memory order.  SCALED: the workgroups from `row_blocks` on take 128 keys of a key head each and find their largest |v_j| (finite ones: a row
+// cancels: with the rounded o, a row of few keys had twice the error of its products' operands); `lanes` lanes (the power of two that covers a
+// row's 16-byte chunks) to a row, rows in memory order.  SCALED: the workgroups from `row_blocks` on take 128 keys of a key head each and find their largest |v_j| (finite ones: a row
 // that sees another has no finite gradient anyhow)
 template <typename T>
 __global__ __launch_bounds__(256) void icg_attention_rowstat_kernel(AttnP p, float* stat, int lanes, int64_t row_blocks) {

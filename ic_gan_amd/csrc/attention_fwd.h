@@ -18,12 +18,14 @@ struct at_fwd_shape {
 };
 
 // Bound and measured.  A SIMD's matrix and vector instructions do not seem to overlap, not even those of its two waves: cycles of the products plus 4
-// for each vector instruction (16 for an exponential) account for 93 - 99 % of a SIMD's busy cycles (counters, fp32 and bf16), and reading
-// operands further ahead, a third wave, or forming the next tile's scores beside the exponentials gained nothing (558 us -> 609 us).  So a
-// lane does per score one fma, one exponential, one add, half a conversion and half a maximum, and nothing else.
-//   2 x 8192 causal, 16 heads of 128 over 4 key heads, bf16:      576 us =  955 TFLOP/s (the library's 8192^3 product: 1234)
-//   64 x 4096 queries, 1024 keys, 48 / 192 elements, fp32:        985 us =  131 TFLOP/s (154)
-//   one token for 32 sequences of 2048 .. 8192 keys, 32 / 8 heads: 154 us = 4.36 TB/s   (a copy: 4.78; two workgroups a unit keep 128 KB in flight)
+// for each vector instruction (16 for an exponential) are 0.92 - 1.02 of a SIMD's busy cycles (counters: fp32, and bf16 at 2 x 8192; 0.88 at
+// 2 x 4096, where the last workgroups leave SIMDs half empty), and reading operands further ahead, a third wave, or forming the next tile's
+// scores beside the exponentials gained nothing (558 us -> 609 us).  So a lane does per score one fma, one exponential, one add, half a
+// conversion and half a maximum, and nothing else.
+//   2 x 8192 causal, 16 heads of 128 over 4 key heads, bf16:      575 us =  956 TFLOP/s (the library's 8192^3 product: 1234)
+//   64 x 4096 queries, 1024 keys, 48 / 192 elements, fp32:        996 us =  129 TFLOP/s (154)
+//   one token for 32 sequences of 2048 .. 8192 keys, 32 / 8 heads: 153 us = 4.4 TB/s   (a copy: 4.78; two workgroups a unit keep 128 KB in flight)
+// One form spills (82 registers, compiled scratch): fp32, few queries, heads of 64 / 256.
 template <typename T, int DP, int DVP, bool TOKENS>
 __global__ __launch_bounds__((at_fwd_shape<T, TOKENS>::THREADS), (at_fwd_shape<T, TOKENS>::template waves<DP, DVP>())) void icg_attention_fwd_kernel(AttnP p) {
   typedef at_fwd_shape<T, TOKENS> S;

@@ -8,8 +8,8 @@
 // part of the sorted list begins; a second sweep puts the positions in place.  Tokens that occur often are summed in pieces of
 // EMB_CHUNK list entries first.  What one wave does in turn still grows with its token: n / EMB_CHUNK sums of pieces for a token that fills
 // the list, and up to EMB_FEW entries, 8 loads at a time, where the list is short and not sorted.
-// Measured, 50000 x 2048 bf16, 16384 skewed tokens: lookup 25 us (5.4 TB/s), order 17 us (the busiest run's entries, one after the other), pieces
-// 13 us, rows 69 us (4.0 TB/s); 1000 x 128 fp32, 64 tokens: 3 us each way.
+// Measured (kernel trace), 50000 x 2048 bf16, 16384 skewed tokens: lookup 24 us (5.6 TB/s), order 16 us (the busiest run's entries, one after the
+// other), pieces 13 us, rows 70 us (4.0 TB/s); 1000 x 128 fp32, 64 tokens: 3 us each way.
 #include "icg_common.h"
 
 typedef unsigned em_u4 __attribute__((ext_vector_type(4)));

@@ -7,8 +7,8 @@
 // per-channel coefficients stay in registers and every row access is whole 16-byte pieces.
 //   one pass     a group's slab [HW][Cg] fits one workgroup's registers (8 rows a thread): read once, normalised from registers
 //   three passes (larger slabs) partial sums of row chunks -> one workgroup per group joins them -> apply; x is read twice
-// Measured, 64 x 256 x 256 x 96 fp32 with ReLU (1.6 GB): first pass 314 us (5.1 TB/s), last 557 us (5.8 TB/s); 32 x 64 x 64 x 384 bf16 with SiLU
-// (100 MB): 36 and 45 us, its gradient 47 and 70 us (4.3 TB/s); 64 x 4 x 4 x 1536 fp32 in one pass: 11 us each way.
+// Measured (kernel trace), 64 x 256 x 256 x 96 fp32 with ReLU (1.6 GB): first pass 327 us (4.9 TB/s), last 565 us (5.7 TB/s); 32 x 64 x 64 x 384
+// bf16 with SiLU (100 MB): 28 and 43 us, its gradient 57 and 66 us (3.6 and 4.5 TB/s); 64 x 4 x 4 x 1536 fp32 in one pass: 10 and 11 us.
 // Means and squared deviations are joined pairwise from sums about each part's own mean (no difference of large squares); across chunks in
 // 64 bits.  All sums in 32 bits or more, in a fixed order, no atomics.
 #include "icg_common.h"

@@ -794,7 +794,8 @@ int icg_sg2_torgb_bwd(const float* dimg, const void* y, const void* x, const flo
  * rounded o).
  * dtype 0 / 1 / 2: fp32 / fp16 / bf16 (matrix products in that type, everything else in fp32).  k_lens, q_start: int32 [B] on the device or
  * NULL (Lk; Lk - Lq); keys from k_lens[b] on are not read, and their dk, dv are zero.  scale > 0.  `_applies`: d, dv <= 128, or d <= 64 and
- * dv <= 256, rows of whole 16-byte chunks.  A non-finite value that the causal mask hides from a query can still reach it (0 * inf); one from k_lens[b] on cannot. */
+ * dv <= 256, rows of whole 16-byte chunks.  A non-finite value that the causal mask hides from a query can still reach it (0 * inf) if a query of
+ * its tile sees it; one from k_lens[b] on cannot. */
 int icg_attention_applies(int B, int Lq, int Lk, int H, int Hk, int d, int dv, int dtype);
 size_t icg_attention_fwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hk, int d, int dv, int dtype);
 int icg_attention_fwd(const void* q, const void* k, const void* v, const int* k_lens, const int* q_start, void* o, void* o_low, float* lse,
